@@ -280,6 +280,99 @@ kmoe_status kmoe_expert_down(const kmoe_desc* desc, const void* h_sorted, const 
 kmoe_status kmoe_combine(const kmoe_desc* desc, const void* y_sorted, const int32_t* inv, const float* topk_w,
                          void* out, void* stream);
 
+/* The residual's addition and the norm that follows it, as one pass
+ * (kappa/qwen3/block.py:71, 153, 196 with norms.py:10-16):
+ *   h   = round(x + residual)               [T,D] activation dtype
+ *   out = kmoe_rms_norm(h), bit for bit     [T,D] activation dtype
+ * h_out may be x or residual itself (in place); the buffers overlap in no other way. */
+kmoe_status kmoe_add_rms_norm(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,
+                              kmoe_dtype scale_dtype, float epsilon, void* h_out, void* out, void* stream);
+
+/* The same with the normalised rows in 8 bits: with v = (h * r) * scale in f32 (not rounded
+ * to the activation dtype) and m the row's largest |v|,
+ *   q_scale[t] = max(m / 127, FLT_MIN),  q = clip(rint(v * (1 / q_scale)), -127, 127).
+ * A row that holds an infinity or a NaN has q_scale = NaN and q = 0, so whatever is
+ * computed from it is NaN. residual and h_out may both be NULL: h = x. */
+kmoe_status kmoe_add_rms_norm_q8(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,
+                                 kmoe_dtype scale_dtype, float epsilon, void* h_out, int8_t* q, float* q_scale,
+                                 void* stream);
+
+/* --- projections ----------------------------------------------------------- */
+/* A projection's weights [in, out] (bf16, or int8 with one scale or one per output
+ * channel), laid out once for the MFMA kernels and padded with zeros: `in` to a multiple
+ * of 128, `out` to one of 32. Both buffers are caller-owned device memory of the
+ * sizes kmoe_linear_pack_bytes() reports:
+ *   values  BF16  [out/16][in/64][2][4][16][8]   [a][b][c][d][e][f]: column 16 a + e, k = 64 b + 16 d + 8 c + f
+ *           I8    [out/16][in/16][16][16]        [a][b][c][d]: column 16 a + c, k = 16 b + d
+ *   scale   f32   [out]                          1 for BF16; a scalar is repeated */
+typedef struct kmoe_linear_weight {
+  void* values;
+  float* scale;
+  kmoe_dtype dtype;      /* BF16 or I8 */
+  int64_t in_features;   /* the matrix's own sizes, without padding */
+  int64_t out_features;
+} kmoe_linear_weight;
+
+/* Low-rank adapters of one projection, laid out once like its weights: a[l] as a BF16
+ * matrix [in, rank] (rank padded to a multiple of 32), b[l] as
+ *   [out/16][rank/32][4][16][8]   [a][b][c][d][e]: column 16 a + d, r = 32 b + 8 c + e
+ * and factor [num_adapters] f32 (an adapter's alpha / rank). */
+typedef struct kmoe_lora {
+  void* a;
+  void* b;
+  float* factor;
+  int64_t num_adapters;
+  int64_t rank;          /* the largest rank of the adapters; smaller ones are padded with zeros */
+  int64_t in_features;
+  int64_t out_features;
+} kmoe_lora;
+
+/* Which adapter each token of a step uses, and the tokens sorted by it (kmoe_lora_sort):
+ *   adapter [T]               the token's adapter, -1 for none
+ *   order   [T]               the tokens by adapter, those without one last, in their order
+ *   sorted  [T]               adapter[order[i]]
+ *   offsets [num_adapters+1]  the adapters' ranges in order */
+typedef struct kmoe_lora_batch {
+  int32_t* adapter;
+  int32_t* order;
+  int32_t* sorted;
+  int32_t* offsets;
+  int64_t tokens;
+  int64_t num_adapters;
+} kmoe_lora_batch;
+
+/* Bytes of the two buffers of a kmoe_linear_weight (its dtype and sizes given). */
+kmoe_status kmoe_linear_pack_bytes(const kmoe_linear_weight* packed, size_t* values_bytes, size_t* scale_bytes);
+/* Lays `w` ([in, out] row-major: BF16, or I8 with a TENSOR scale or a CHANNEL scale [out])
+ * out into `packed`. */
+kmoe_status kmoe_linear_pack(const kmoe_weight* w, const kmoe_linear_weight* packed, void* stream);
+/* Bytes of the buffers a and b of a kmoe_lora (its sizes given; factor holds num_adapters floats). */
+kmoe_status kmoe_lora_pack_bytes(const kmoe_lora* lora, size_t* a_bytes, size_t* b_bytes);
+/* Lays `count` adapters of one rank <= lora->rank (a [count, in, rank] and b [count, rank, out],
+ * BF16, row-major; factor [count] f32) out into the slots first .. first + count - 1. The
+ * other slots keep what they hold. */
+kmoe_status kmoe_lora_pack(const kmoe_lora* lora, int64_t first, int64_t count, int64_t rank, const void* a,
+                           const void* b, const float* factor, void* stream);
+/* Fills `batch` from adapter [T] int32: a value outside [0, num_adapters) means none. Needed
+ * once for a step; every projection of the step takes the same batch. scratch: kmoe_lora_sort_bytes(). */
+kmoe_status kmoe_lora_sort_bytes(const kmoe_lora_batch* batch, size_t* bytes);
+kmoe_status kmoe_lora_sort(const int32_t* adapter, const kmoe_lora_batch* batch, void* scratch, size_t scratch_bytes,
+                           void* stream);
+
+/* Bytes of device workspace kmoe_linear needs for up to `tokens` rows of x_dtype (lora may be NULL). */
+kmoe_status kmoe_linear_workspace_bytes(const kmoe_linear_weight* w, int64_t tokens, kmoe_dtype x_dtype,
+                                        const kmoe_lora* lora, size_t* bytes);
+/* out[t] = round(x_scale[t] * w.scale * (x[t] @ w.values) [+ u[t] @ b[a]]),
+ * u[t] = factor[a] * x_scale[t] * (x[t] @ a[a]) with a = batch->adapter[t] (nothing is added for -1).
+ *   x       [T, in], rows x_stride elements apart: BF16 (x_scale NULL: 1), or I8 with
+ *           x_scale [T] f32 (kmoe_add_rms_norm_q8's outputs), which takes I8 weights
+ *   out     [T, out] BF16
+ * Sums in f32 (int8 rows: exact in i32 first); u stays f32 up to 64 tokens and is carried as
+ * bf16(u) + bf16(u - bf16(u)) above. lora and batch are both NULL or both given. x spans less than 4 GiB. */
+kmoe_status kmoe_linear(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                        int64_t x_stride, const float* x_scale, const kmoe_lora* lora, const kmoe_lora_batch* batch,
+                        void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* --- weights -------------------------------------------------------------- */
 /* Relayout gate/up/down ([E,D,I], [E,I,D]; int8 + per-tensor or per-channel
  * scale) into `packed` for the gfx950 kernels. */

@@ -59,6 +59,16 @@ EXPORTS = (
     "kmoe_forward_noalloc",
     "kmoe_forward_block",
     "kmoe_rms_norm",
+    "kmoe_add_rms_norm",
+    "kmoe_add_rms_norm_q8",
+    "kmoe_linear_pack_bytes",
+    "kmoe_linear_pack",
+    "kmoe_lora_pack_bytes",
+    "kmoe_lora_pack",
+    "kmoe_lora_sort_bytes",
+    "kmoe_lora_sort",
+    "kmoe_linear_workspace_bytes",
+    "kmoe_linear",
     "kmoe_route",
     "kmoe_route_scratch_bytes",
     "kmoe_dispatch",
@@ -119,6 +129,39 @@ class KmoePackedSizes(ctypes.Structure):
     ]
 
 
+class KmoeLinear(ctypes.Structure):
+    _fields_ = [
+        ("values", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("in_features", ctypes.c_int64),
+        ("out_features", ctypes.c_int64),
+    ]
+
+
+class KmoeLora(ctypes.Structure):
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("factor", ctypes.c_void_p),
+        ("num_adapters", ctypes.c_int64),
+        ("rank", ctypes.c_int64),
+        ("in_features", ctypes.c_int64),
+        ("out_features", ctypes.c_int64),
+    ]
+
+
+class KmoeLoraBatch(ctypes.Structure):
+    _fields_ = [
+        ("adapter", ctypes.c_void_p),
+        ("order", ctypes.c_void_p),
+        ("sorted", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("num_adapters", ctypes.c_int64),
+    ]
+
+
 class KmoeError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(message)
@@ -132,6 +175,10 @@ _P = ctypes.c_void_p
 _WP = ctypes.POINTER(KmoeWeight)
 _DP = ctypes.POINTER(KmoeDesc)
 _PP = ctypes.POINTER(KmoePacked)
+_LP = ctypes.POINTER(KmoeLinear)
+_RP = ctypes.POINTER(KmoeLora)
+_BP = ctypes.POINTER(KmoeLoraBatch)
+_ZP = ctypes.POINTER(ctypes.c_size_t)
 
 
 def _declare(L: ctypes.CDLL) -> None:
@@ -169,6 +216,28 @@ def _declare(L: ctypes.CDLL) -> None:
     L.kmoe_expert_down.argtypes = [_DP, _P, _P, _P, _P, _WP, _PP, _P, _P]
     L.kmoe_combine.restype = ctypes.c_int
     L.kmoe_combine.argtypes = [_DP, _P, _P, _P, _P, _P]
+    L.kmoe_add_rms_norm.restype = ctypes.c_int
+    L.kmoe_add_rms_norm.argtypes = [_DP, _P, _P, _P, ctypes.c_int, ctypes.c_float, _P, _P, _P]
+    L.kmoe_add_rms_norm_q8.restype = ctypes.c_int
+    L.kmoe_add_rms_norm_q8.argtypes = [_DP, _P, _P, _P, ctypes.c_int, ctypes.c_float, _P, _P, _P, _P]
+    L.kmoe_linear_pack_bytes.restype = ctypes.c_int
+    L.kmoe_linear_pack_bytes.argtypes = [_LP, _ZP, _ZP]
+    L.kmoe_linear_pack.restype = ctypes.c_int
+    L.kmoe_linear_pack.argtypes = [_WP, _LP, _P]
+    L.kmoe_lora_pack_bytes.restype = ctypes.c_int
+    L.kmoe_lora_pack_bytes.argtypes = [_RP, _ZP, _ZP]
+    L.kmoe_lora_pack.restype = ctypes.c_int
+    L.kmoe_lora_pack.argtypes = [_RP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P, _P, _P, _P]
+    L.kmoe_lora_sort_bytes.restype = ctypes.c_int
+    L.kmoe_lora_sort_bytes.argtypes = [_BP, _ZP]
+    L.kmoe_lora_sort.restype = ctypes.c_int
+    L.kmoe_lora_sort.argtypes = [_P, _BP, _P, ctypes.c_size_t, _P]
+    L.kmoe_linear_workspace_bytes.restype = ctypes.c_int
+    L.kmoe_linear_workspace_bytes.argtypes = [_LP, ctypes.c_int64, ctypes.c_int, _RP, _ZP]
+    L.kmoe_linear.restype = ctypes.c_int
+    L.kmoe_linear.argtypes = [
+        _LP, ctypes.c_int64, _P, ctypes.c_int, ctypes.c_int64, _P, _RP, _BP, _P, _P, ctypes.c_size_t, _P,
+    ]  # fmt: skip
     L.kmoe_prepack.restype = ctypes.c_int
     L.kmoe_prepack.argtypes = [_DP, _WP, _WP, _WP, _PP, _P]
     L.kmoe_to_compute_dtype.restype = ctypes.c_int

@@ -349,6 +349,29 @@ kmoe_status kmoe_rms_norm(const kmoe_desc* desc, const void* x, const void* scal
   return KMOE_OK;
 }
 
+kmoe_status kmoe_add_rms_norm(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,
+                              kmoe_dtype scale_dtype, float epsilon, void* h_out, void* out, void* stream) {
+  KMOE_TRY(validate_add_rms_norm(desc, x, residual, scale, scale_dtype, epsilon, h_out, out));
+  KMOE_TRY(device_status());
+  if (desc->tokens == 0) return KMOE_OK;
+  KMOE_HIP(launch_add_rms_norm(*desc, x, residual, scale, scale_dtype, epsilon, h_out, out, nullptr, nullptr,
+                               (hipStream_t)stream),
+           "add_rms_norm kernel");
+  return KMOE_OK;
+}
+
+kmoe_status kmoe_add_rms_norm_q8(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,
+                                 kmoe_dtype scale_dtype, float epsilon, void* h_out, int8_t* q, float* q_scale,
+                                 void* stream) {
+  KMOE_TRY(validate_add_rms_norm_q8(desc, x, residual, scale, scale_dtype, epsilon, h_out, q, q_scale));
+  KMOE_TRY(device_status());
+  if (desc->tokens == 0) return KMOE_OK;
+  KMOE_HIP(launch_add_rms_norm(*desc, x, residual, scale, scale_dtype, epsilon, h_out, nullptr, q, q_scale,
+                               (hipStream_t)stream),
+           "add_rms_norm_q8 kernel");
+  return KMOE_OK;
+}
+
 kmoe_status kmoe_forward_block(const kmoe_desc* desc, const void* h, const void* norm_scale, kmoe_dtype norm_dtype,
                                float epsilon, const kmoe_weight* router, const kmoe_weight* gate,
                                const kmoe_weight* up, const kmoe_weight* down, const kmoe_packed_experts* packed,

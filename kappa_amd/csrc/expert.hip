@@ -49,21 +49,6 @@ __device__ __forceinline__ void dequant16(const uint4 q, const float s, bf16x8& 
   hi = __builtin_bit_cast(bf16x8, uint4{o[4], o[5], o[6], o[7]});
 }
 
-// 16 int8 -> the same 16 integers in bf16 (exact: |q| <= 128 needs 8 bits), for the
-// f32 chain, which applies its f32 scale to the sum
-__device__ __forceinline__ void cvt16(const uint4 q, bf16x8& lo, bf16x8& hi) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  uint32_t o[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t v = w[j >> 1];
-    const int sh = 16 * (j & 1);
-    o[j] = pack_bf16x2((float)(int8_t)((v >> sh) & 0xffu), (float)(int8_t)((v >> (sh + 8)) & 0xffu));
-  }
-  lo = __builtin_bit_cast(bf16x8, uint4{o[0], o[1], o[2], o[3]});
-  hi = __builtin_bit_cast(bf16x8, uint4{o[4], o[5], o[6], o[7]});
-}
-
 // The B operand of a 16-byte int8 load for chain CH: bf16(q * s) with s already
 // rounded to bf16 (kChainAct), or the exact integers (kChainF32).
 template <int CH>

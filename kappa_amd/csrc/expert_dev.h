@@ -27,6 +27,21 @@ __device__ __forceinline__ void transpose2(const uint32_t* r, bf16x8& c0, bf16x8
   c1 = as_bf16x8(uint4{pair_hi(r[0], r[1]), pair_hi(r[2], r[3]), pair_hi(r[4], r[5]), pair_hi(r[6], r[7])});
 }
 
+// 16 int8 -> the same 16 integers in bf16 (exact: |q| <= 128 needs 8 bits), for a
+// product whose f32 scale is applied to the sum
+__device__ __forceinline__ void cvt16(const uint4 q, bf16x8& lo, bf16x8& hi) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t v = w[j >> 1];
+    const int sh = 16 * (j & 1);
+    o[j] = pack_bf16x2((float)(int8_t)((v >> sh) & 0xffu), (float)(int8_t)((v >> (sh + 8)) & 0xffu));
+  }
+  lo = __builtin_bit_cast(bf16x8, uint4{o[0], o[1], o[2], o[3]});
+  hi = __builtin_bit_cast(bf16x8, uint4{o[4], o[5], o[6], o[7]});
+}
+
 // 16 bytes with a nontemporal load: for data a kernel reads exactly once, such
 // as the decode weights (streaming reads this way sustain ~7.1 TB/s on MI355X
 // against ~6.3 TB/s for ordinary loads, which also allocate in the caches)

@@ -478,6 +478,34 @@ kmoe_status validate_rms_norm(const kmoe_desc* desc, const void* x, const void* 
   return KMOE_OK;
 }
 
+kmoe_status validate_add_rms_norm(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,
+                                  kmoe_dtype scale_dtype, float epsilon, const void* h_out, const void* out) {
+  KMOE_TRY(check_desc(desc));
+  KMOE_TRY(check_norm_args(scale, scale_dtype, epsilon));
+  if (desc->tokens == 0) return KMOE_OK;
+  if (!x || !residual || !h_out || !out)
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_add_rms_norm: x, residual, h_out and out must be non-NULL");
+  if (out == x || out == residual || out == h_out)
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_add_rms_norm: out must not alias x, residual or h_out");
+  return KMOE_OK;
+}
+
+kmoe_status validate_add_rms_norm_q8(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,
+                                     kmoe_dtype scale_dtype, float epsilon, const void* h_out, const int8_t* q,
+                                     const float* q_scale) {
+  KMOE_TRY(check_desc(desc));
+  KMOE_TRY(check_norm_args(scale, scale_dtype, epsilon));
+  if (!residual != !h_out)
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_add_rms_norm_q8: residual and h_out come together");
+  if (desc->tokens == 0) return KMOE_OK;
+  if (!x || !q || !q_scale)
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_add_rms_norm_q8: x, q and q_scale must be non-NULL");
+  const void* o = q;
+  if (o == x || o == residual || o == h_out)
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_add_rms_norm_q8: q must not alias x, residual or h_out");
+  return KMOE_OK;
+}
+
 kmoe_status validate_prepack(const kmoe_desc* desc, const kmoe_weight* gate, const kmoe_weight* up,
                              const kmoe_weight* down, const kmoe_packed_experts* packed) {
   KMOE_TRY(check_desc(desc));

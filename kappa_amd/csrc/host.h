@@ -214,6 +214,12 @@ kmoe_status validate_combine(const kmoe_desc* desc, const void* y_sorted, const 
                              const void* out);
 kmoe_status validate_rms_norm(const kmoe_desc* desc, const void* x, const void* scale, kmoe_dtype scale_dtype,
                               float epsilon, const void* out);
+// add_rms_norm: out given; add_rms_norm_q8: q and q_scale
+kmoe_status validate_add_rms_norm(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,
+                                  kmoe_dtype scale_dtype, float epsilon, const void* h_out, const void* out);
+kmoe_status validate_add_rms_norm_q8(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,
+                                     kmoe_dtype scale_dtype, float epsilon, const void* h_out, const int8_t* q,
+                                     const float* q_scale);
 kmoe_status validate_prepack(const kmoe_desc* desc, const kmoe_weight* gate, const kmoe_weight* up,
                              const kmoe_weight* down, const kmoe_packed_experts* packed);
 kmoe_status validate_to_compute_dtype(const kmoe_weight* w, int64_t outer, int64_t channels,

@@ -106,6 +106,12 @@ hipError_t launch_gateup_routed(const kmoe_desc& d, int chain, const float* part
 hipError_t launch_rms_norm(const kmoe_desc& d, const void* h, const void* scale, kmoe_dtype scale_dtype, float eps,
                            void* out, hipStream_t st);
 
+// h = x + res and its norm: out, or q and qscale (the other NULL); res and hout may both be
+// NULL with q
+hipError_t launch_add_rms_norm(const kmoe_desc& d, const void* x, const void* res, const void* scale,
+                               kmoe_dtype scale_dtype, float eps, void* hout, void* out, int8_t* q, float* qscale,
+                               hipStream_t st);
+
 // weights.hip
 hipError_t launch_prepack(const kmoe_desc& d, const kmoe_weight& gate, const kmoe_weight& up, const kmoe_weight& down,
                           const kmoe_packed_experts& p, hipStream_t st);

@@ -1,0 +1,829 @@
+// Projections of a decoder layer, y = x W, and the low-rank adapters of many requests
+// beside them: token t of adapter a adds factor_a (x_t A_a) B_a.
+//
+// Reference: the q, k, v and o einsums (kappa/qwen3/linear.py:10-25) over
+// to_compute_dtype weights (kappa/qwen3/quant.py:34-38); it has no adapters. The
+// scale of int8 weights multiplies the f32 sum of the products with the integers, so
+// nothing is rounded between the operands and the output.
+//
+// Three kinds of products (Kind): bf16 rows with bf16 or int8 weights on
+// v_mfma_f32_16x16x32_bf16 (int8 becomes bf16 in registers, exactly), and int8 rows
+// with int8 weights on v_mfma_i32_16x16x64_i8, whose sums are exact.
+#include "common.h"
+#include "expert_dev.h"
+#include "linear_launch.h"
+
+namespace kmoe {
+
+namespace {
+
+constexpr int kBB = 0;  // bf16 rows, bf16 weights
+constexpr int kBI = 1;  // bf16 rows, int8 weights
+constexpr int kII = 2;  // int8 rows, int8 weights
+
+struct LinearArgs {
+  const char* x;      // rows, 16-byte aligned
+  uint32_t row_bytes;
+  const float* xs;    // the rows' scales (kII)
+  const char* w;
+  const float* ws;
+  uint16_t* out;
+  int T, N, kc;       // kc: 64-deep chunks
+  int cgs;            // column groups (16 columns) of the packed weights
+  size_t cg_bytes;    // bytes of one
+  // adapters
+  const int32_t* adapter;  // NULL: none
+  const int32_t* order;
+  const int32_t* sorted;
+  const int32_t* offsets;
+  const char* a;      // [L][rank/16][in/64][2][4][16][8]
+  const char* b;      // [L][out/16][rank/32][4][16][8]
+  const float* factor;
+  int rank, rp, kcp;  // rank, rank padded, 64-deep chunks of the packed A
+  void* u;            // up to 64 tokens f32 [T][rp]; above, bf16 [T][rp/32][hi 32 | lo 32] in sorted order
+};
+
+__device__ __forceinline__ int32x4 as_i32x4(const uint4 v) { return __builtin_bit_cast(int32x4, v); }
+
+__device__ __forceinline__ void unpack8(const uint4 v, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// four output columns of one row; vec: rows on 8-byte boundaries
+__device__ __forceinline__ void store4(uint16_t* __restrict__ row, int col, int N, bool vec, const float* v) {
+  if (vec && col + 4 <= N) {
+    *reinterpret_cast<uint2*>(row + col) = uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (col + j < N) row[col + j] = f32_to_bf16_bits(v[j]);
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// Load time: weights and adapters into the layouts of include/kmoe.h, one 16-byte
+// piece per thread (16 neighbouring threads read 16 neighbouring columns).
+// ---------------------------------------------------------------------------
+
+// bf16 [K][N] (or its `mats` copies, one after the other) -> [N/16][K/64][2][4][16][8], zeros outside
+__global__ __launch_bounds__(256) void k_pack_bf16(int64_t mats, int K, int N, int Kp, int Np,
+                                                   const uint16_t* __restrict__ src, uint16_t* __restrict__ dst) {
+  const int64_t per = (int64_t)Kp * Np / 8;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < mats * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / per, p = i - m * per;
+    const int c = p & 15, q = (p >> 4) & 3, st = (p >> 6) & 1;
+    const int64_t cell = p >> 7;
+    const int kc = (int)(cell % (Kp >> 6)), n = (int)(cell / (Kp >> 6)) * 16 + c;
+    const int k0 = kc * 64 + 16 * q + 8 * st;
+    uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n < N && k0 + j < K) v[j >> 1] |= (uint32_t)src[(m * K + k0 + j) * N + n] << (16 * (j & 1));
+    reinterpret_cast<uint4*>(dst)[i] = uint4{v[0], v[1], v[2], v[3]};
+  }
+}
+
+// int8 [K][N] -> [N/16][K/16][16][16], zeros outside
+__global__ __launch_bounds__(256) void k_pack_i8(int K, int N, int Kp, int Np, const uint8_t* __restrict__ src,
+                                                 uint8_t* __restrict__ dst) {
+  const int64_t pieces = (int64_t)Kp * Np / 16;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
+    const int c = i & 15;
+    const int64_t cell = i >> 4;
+    const int k0 = (int)(cell % (Kp >> 4)) * 16, n = (int)(cell / (Kp >> 4)) * 16 + c;
+    uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (n < N && k0 + j < K) v[j >> 2] |= (uint32_t)src[(int64_t)(k0 + j) * N + n] << (8 * (j & 3));
+    reinterpret_cast<uint4*>(dst)[i] = uint4{v[0], v[1], v[2], v[3]};
+  }
+}
+
+// the scales of N columns in f32; kind: kmoe_scale_kind
+__global__ __launch_bounds__(256) void k_pack_scale(int N, int Np, int kind, int s_bf16, const void* __restrict__ s,
+                                                    float* __restrict__ dst) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= Np) return;
+  float v = 1.0f;
+  if (kind != KMOE_SCALE_NONE) {
+    const int i = kind == KMOE_SCALE_CHANNEL ? min(n, N - 1) : 0;
+    v = s_bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(s)[i]) : reinterpret_cast<const float*>(s)[i];
+  }
+  dst[n] = v;
+}
+
+// B [count][R][N] -> slots of [N/16][rp/32][4][16][8], zeros outside
+__global__ __launch_bounds__(256) void k_pack_lora_b(int64_t count, int R, int N, int rp, int Np,
+                                                     const uint16_t* __restrict__ src, uint16_t* __restrict__ dst) {
+  const int64_t per = (int64_t)rp * Np / 8;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / per, p = i - m * per;
+    const int c = p & 15, r8 = (p >> 4) & 3;
+    const int64_t cell = p >> 6;
+    const int r0 = (int)(cell % (rp >> 5)) * 32 + 8 * r8, n = (int)(cell / (rp >> 5)) * 16 + c;
+    uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n < N && r0 + j < R) v[j >> 1] |= (uint32_t)src[(m * R + r0 + j) * N + n] << (16 * (j & 1));
+    reinterpret_cast<uint4*>(dst)[i] = uint4{v[0], v[1], v[2], v[3]};
+  }
+}
+
+__global__ __launch_bounds__(256) void k_copy_f32(int64_t n, const float* __restrict__ src, float* __restrict__ dst) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) dst[i] = src[i];
+}
+
+// Rows that the kernels cannot read where they are (a width that is no multiple of a
+// step, rows off 16-byte boundaries): copied, the width filled up with zeros.
+template <typename E>
+__global__ __launch_bounds__(256) void k_stage_rows(int64_t T, int K, int Kp, int64_t stride,
+                                                    const E* __restrict__ src, E* __restrict__ dst) {
+  const int64_t n = T * Kp;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / Kp;
+    const int k = (int)(i - t * Kp);
+    dst[i] = k < K ? src[t * stride + k] : (E)0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The tokens of a step by adapter: a stable counting sort over L + 1 buckets (the
+// last: no adapter). Blocks of 512 tokens count themselves (k_lora_count, not needed for one
+// block); then every block adds up the counts and ranks its own tokens: inside a wave
+// by matching the buckets' bits, the waves by their counts in LDS.
+// ---------------------------------------------------------------------------
+namespace {
+
+__device__ __forceinline__ int lora_bucket(const int32_t* __restrict__ adapter, int64_t t, int64_t T, int L) {
+  if (t >= T) return -1;
+  const int a = adapter[t];
+  return a >= 0 && a < L ? a : L;
+}
+
+}  // namespace
+
+__global__ __launch_bounds__(kLoraSortBlock) void k_lora_count(int T, int L, const int32_t* __restrict__ adapter,
+                                                               int32_t* __restrict__ hist) {
+  __shared__ int cnt[kLoraMaxAdapters + 1];
+  for (int i = threadIdx.x; i <= L; i += kLoraSortBlock) cnt[i] = 0;
+  __syncthreads();
+  const int b = lora_bucket(adapter, (int64_t)blockIdx.x * kLoraSortBlock + threadIdx.x, T, L);
+  if (b >= 0) atomicAdd(&cnt[b], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i <= L; i += kLoraSortBlock) hist[(int64_t)blockIdx.x * (L + 1) + i] = cnt[i];
+}
+
+__global__ __launch_bounds__(kLoraSortBlock) void k_lora_sort(int T, int L, const int32_t* __restrict__ adapter,
+                                                              const int32_t* __restrict__ hist, int blocks,
+                                                              int32_t* __restrict__ row_adapter,
+                                                              int32_t* __restrict__ order,
+                                                              int32_t* __restrict__ sorted,
+                                                              int32_t* __restrict__ offsets) {
+  constexpr int kWaves = kLoraSortBlock / 64;
+  __shared__ int cnt[kWaves][kLoraMaxAdapters + 1];  // a wave's tokens of a bucket; then where its first goes
+  __shared__ int total[kLoraMaxAdapters + 1];        // tokens of a bucket; then its start
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  for (int i = tid; i < kWaves * (kLoraMaxAdapters + 1); i += kLoraSortBlock) (&cnt[0][0])[i] = 0;
+  __syncthreads();
+  const int64_t t = (int64_t)blockIdx.x * kLoraSortBlock + tid;
+  const int b = lora_bucket(adapter, t, T, L);
+  // the lanes with the same bucket (11 bits; those past the batch match each other)
+  uint64_t same = ~0ull;
+  for (int bit = 0; bit < 11; ++bit) {
+    const uint64_t m = __ballot((b >> bit) & 1);
+    same &= ((b >> bit) & 1) ? m : ~m;
+  }
+  const int rank = __popcll(same & ((1ull << lane) - 1));
+  if (b >= 0 && rank == 0) cnt[wv][b] = __popcll(same);
+  __syncthreads();
+  // per bucket: the tokens of the blocks before this one, of all blocks, and of this one's waves
+  for (int i = tid; i <= L; i += kLoraSortBlock) {
+    int before = 0, all = 0;
+    if (blocks > 1) {
+      for (int k = 0; k < blocks; ++k) {
+        const int h = hist[(int64_t)k * (L + 1) + i];
+        if (k < (int)blockIdx.x) before += h;
+        all += h;
+      }
+    }
+    int run = before;
+    for (int w = 0; w < kWaves; ++w) {
+      const int h = cnt[w][i];
+      cnt[w][i] = run;
+      run += h;
+    }
+    total[i] = blocks > 1 ? all : run;
+  }
+  __syncthreads();
+  // the buckets' starts: one wave, 64 buckets at a time
+  if (wv == 0) {
+    int base = 0;
+    for (int i0 = 0; i0 <= L; i0 += 64) {
+      const int i = i0 + lane;
+      const int v = i <= L ? total[i] : 0;
+      int incl = v;
+      for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += o;
+      }
+      if (i <= L) total[i] = base + incl - v;
+      base += __shfl(incl, 63, 64);
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= L; i += kLoraSortBlock) offsets[i] = total[i];
+  if (b < 0) return;
+  const int at = total[b] + cnt[wv][b] + rank;
+  const int a = b < L ? b : -1;
+  row_adapter[t] = a;
+  order[at] = (int32_t)t;
+  sorted[at] = a;
+}
+
+// ---------------------------------------------------------------------------
+// u = factor x A for few tokens: one block per token and 16 ranks, 16 waves over the chunks.
+// ---------------------------------------------------------------------------
+template <int KIND>
+__global__ __launch_bounds__(1024) void k_lora_shrink_rows(LinearArgs p) {
+  __shared__ float red[16][16];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q = lane >> 4;
+  const int t = blockIdx.x, g = blockIdx.y;
+  const int ad = p.adapter[t];
+  if (ad < 0) return;  // the whole block
+  const char* xr = p.x + (size_t)t * p.row_bytes + q * (KIND == kII ? 16 : 32);
+  const char* ar = p.a + (size_t)ad * p.rp * p.kcp * 128 + (size_t)g * p.kcp * 2048 + lane * 16;
+  float acc = 0.0f;
+  for (int kc = wv; kc < p.kc; kc += 16) {
+    const uint4 a0 = *reinterpret_cast<const uint4*>(ar + (size_t)kc * 2048);
+    const uint4 a1 = *reinterpret_cast<const uint4*>(ar + (size_t)kc * 2048 + 1024);
+    float fa[16], fx[16];
+    unpack8(a0, fa);
+    unpack8(a1, fa + 8);
+    if constexpr (KIND == kII) {
+      const uint4 v = *reinterpret_cast<const uint4*>(xr + kc * 64);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) fx[j] = (float)(int8_t)((w[j >> 2] >> (8 * (j & 3))) & 0xffu);
+    } else {
+      unpack8(*reinterpret_cast<const uint4*>(xr + kc * 128), fx);
+      unpack8(*reinterpret_cast<const uint4*>(xr + kc * 128 + 16), fx + 8);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc = __builtin_fmaf(fx[j], fa[j], acc);
+  }
+  acc += __shfl_xor(acc, 16, 64);
+  acc += __shfl_xor(acc, 32, 64);
+  if (lane < 16) red[wv][lane] = acc;
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    float s = 0.0f;
+    for (int w = 0; w < 16; ++w) s += red[w][threadIdx.x];
+    s *= p.factor[ad];
+    if (KIND == kII) s *= p.xs[t];
+    reinterpret_cast<float*>(p.u)[(size_t)t * p.rp + g * 16 + threadIdx.x] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// u for many tokens, 16 sorted rows per block: MFMA, eight waves over the chunks, one
+// pass per adapter of the tile; u as bf16 hi + lo.
+// ---------------------------------------------------------------------------
+template <int KIND>
+__global__ __launch_bounds__(512) void k_lora_shrink(LinearArgs p) {
+  constexpr int NG = 4;  // groups of 16 ranks at a time
+  __shared__ floatx4 red[8][NG][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
+  const int r0 = blockIdx.x * 16, r1 = min(r0 + 16, p.T);
+  const int row = p.order[min(r0 + c, p.T - 1)];
+  const char* xr = p.x + (size_t)row * p.row_bytes + q * (KIND == kII ? 16 : 32);
+  const float xs = KIND == kII ? p.xs[row] : 1.0f;
+  const int groups = p.rp >> 4;
+  for (int pos = r0; pos < r1;) {
+    const int ad = p.sorted[pos];
+    if (ad < 0) break;
+    const int end = min(max(p.offsets[ad + 1], pos + 1), r1);
+    const float f = p.factor[ad];
+    for (int g0 = 0; g0 < groups; g0 += NG) {
+      const char* ar = p.a + (size_t)ad * p.rp * p.kcp * 128 + (size_t)g0 * p.kcp * 2048 + lane * 16;
+      floatx4 acc[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) acc[g] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int kc = wv; kc < p.kc; kc += 8) {
+        bf16x8 x0, x1;
+        if constexpr (KIND == kII) {
+          cvt16(*reinterpret_cast<const uint4*>(xr + kc * 64), x0, x1);
+        } else {
+          x0 = as_bf16x8(*reinterpret_cast<const uint4*>(xr + kc * 128));
+          x1 = as_bf16x8(*reinterpret_cast<const uint4*>(xr + kc * 128 + 16));
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          if (g0 + g < groups) {
+            const char* at = ar + ((size_t)g * p.kcp + kc) * 2048;
+            acc[g] = mfma16(as_bf16x8(*reinterpret_cast<const uint4*>(at)), x0, acc[g]);
+            acc[g] = mfma16(as_bf16x8(*reinterpret_cast<const uint4*>(at + 1024)), x1, acc[g]);
+          }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) red[wv][g][lane] = acc[g];
+      __syncthreads();
+      if (wv < NG && g0 + wv < groups && r0 + c >= pos && r0 + c < end) {
+        floatx4 s = red[0][wv][lane];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) s += red[w][wv][lane];
+        // ranks 4 q .. 4 q + 3 of group g0 + wv
+        const int r = (g0 + wv) * 16 + 4 * q;
+        uint16_t* u = reinterpret_cast<uint16_t*>(p.u) + (size_t)(r0 + c) * p.rp * 2 + (r >> 5) * 64 + (r & 31);
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_bf16(s[j] * xs * f, hi[j], lo[j]);
+        *reinterpret_cast<uint2*>(u) = uint2{hi[0] | (uint32_t)hi[1] << 16, hi[2] | (uint32_t)hi[3] << 16};
+        *reinterpret_cast<uint2*>(u + 32) = uint2{lo[0] | (uint32_t)lo[1] << 16, lo[2] | (uint32_t)lo[3] << 16};
+      }
+      __syncthreads();
+    }
+    pos = end;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 64 tokens: the weights stream through registers once. A block takes 16 CG
+// columns for all rows, its eight waves the chunks in turn parts; the partial sums meet
+// in LDS in wave order. Each thread then finishes four columns of a row, with the
+// adapters' part in f32.
+// ---------------------------------------------------------------------------
+template <int KIND, int RB, int CG>
+__global__ __launch_bounds__(512) void k_linear_decode(LinearArgs p) {
+  constexpr int NB = 2;
+  constexpr int WL = KIND == kBB ? 2 : 1;   // 16-byte weight loads per chunk and group
+  constexpr int XL = KIND == kII ? 1 : 2;   // and row loads per chunk and row block
+  __shared__ floatx4 red[8][CG][RB][64];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, q = lane >> 4;
+  const char* wb[CG];
+#pragma unroll
+  for (int g = 0; g < CG; ++g)
+    wb[g] = p.w + (size_t)min((int)blockIdx.x * CG + g, p.cgs - 1) * p.cg_bytes + lane * 16;
+  const char* xr[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+    xr[b] = p.x + (size_t)min(b * 16 + c, p.T - 1) * p.row_bytes + q * (16 * XL);
+  floatx4 acc[CG][RB];
+  int32x4 iacc[CG][RB];
+#pragma unroll
+  for (int g = 0; g < CG; ++g)
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      acc[g][b] = floatx4{0.f, 0.f, 0.f, 0.f};
+      iacc[g][b] = int32x4{0, 0, 0, 0};
+    }
+  const int c0 = p.kc * wv / 8, c1 = p.kc * (wv + 1) / 8;
+  for (int cb = c0; cb < c1; cb += NB) {
+    uint4 w[NB][CG][WL], x[NB][RB][XL];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      if (cb + i < c1) {
+#pragma unroll
+        for (int g = 0; g < CG; ++g)
+#pragma unroll
+          for (int l = 0; l < WL; ++l)
+            w[i][g][l] = load_stream16(reinterpret_cast<const int8_t*>(wb[g]) + (size_t)(cb + i) * (1024 * WL) + l * 1024);
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int l = 0; l < XL; ++l)
+            x[i][b][l] = *reinterpret_cast<const uint4*>(xr[b] + (cb + i) * (64 * XL) + l * 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      if (cb + i < c1) {
+#pragma unroll
+        for (int g = 0; g < CG; ++g) {
+          if constexpr (KIND == kII) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+              iacc[g][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as_i32x4(w[i][g][0]), as_i32x4(x[i][b][0]), iacc[g][b],
+                                                                 0, 0, 0);
+          } else {
+            bf16x8 lo, hi;
+            if constexpr (KIND == kBI) {
+              cvt16(w[i][g][0], lo, hi);
+            } else {
+              lo = as_bf16x8(w[i][g][0]);
+              hi = as_bf16x8(w[i][g][WL - 1]);
+            }
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+              acc[g][b] = mfma16(lo, as_bf16x8(x[i][b][0]), acc[g][b]);
+              acc[g][b] = mfma16(hi, as_bf16x8(x[i][b][XL - 1]), acc[g][b]);
+            }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < CG; ++g)
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+      red[wv][g][b][lane] = KIND == kII ? __builtin_bit_cast(floatx4, iacc[g][b]) : acc[g][b];
+  __syncthreads();
+  if (wv >= CG * RB) return;
+  const int g = wv / RB, b = wv % RB;
+  const int row = b * 16 + c, cg = blockIdx.x * CG + g, col = cg * 16 + 4 * q;
+  if (row >= p.T || cg >= p.cgs) return;
+  float v[4];
+  const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + col);
+  if constexpr (KIND == kII) {
+    int32x4 s = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += __builtin_bit_cast(int32x4, red[w][g][b][lane]);
+    const float xs = p.xs[row];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (float)s[j] * xs * sc[j];
+  } else {
+    floatx4 s = red[0][g][b][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) s += red[w][g][b][lane];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = s[j] * sc[j];
+  }
+  if (p.adapter) {
+    const int ad = p.adapter[row];
+    if (ad >= 0) {
+      const float* u = reinterpret_cast<const float*>(p.u) + (size_t)row * p.rp;
+      const char* bb = p.b + ((size_t)ad * p.cgs + cg) * (p.rp * 32) + q * 64;
+      for (int r = 0; r < p.rank; r += 8) {
+        const floatx4 u0 = *reinterpret_cast<const floatx4*>(u + r), u1 = *reinterpret_cast<const floatx4*>(u + r + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float f[8];
+          unpack8(*reinterpret_cast<const uint4*>(bb + r * 32 + j * 16), f);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[j] = __builtin_fmaf(u0[k], f[k], v[j]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[j] = __builtin_fmaf(u1[k], f[4 + k], v[j]);
+        }
+      }
+    }
+  }
+  store4(p.out + (size_t)row * p.N, col, p.N, (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0, v);
+}
+
+// ---------------------------------------------------------------------------
+// Above 64 tokens: a GEMM over tiles of BM rows and BN columns. Steps of 128 bytes of
+// every row (64 bf16, 128 int8) and the columns' weights of the same depth reach LDS by direct
+// loads, two stages. Rows as [row][8 x 16 B] with the pieces swizzled by row
+// (a_piece_at), the weights in the packed order, which is the order their lanes read. The
+// weights are the MFMA's first operand: a lane ends with four consecutive columns.
+//
+// With adapters the rows are the sorted ones, so a tile meets few adapters. After the
+// base sum, already scaled to f32, each adapter of the tile adds steps of 32 ranks: the
+// tile's rows of u (hi and lo, 128 bytes) times the adapter's B. A 16-row group that lies
+// wholly in the adapter's range adds in place; one that does not computes the product
+// apart and takes its own rows by selection, so that nothing of another adapter (an infinity
+// times zero) reaches a row.
+// ---------------------------------------------------------------------------
+template <int KIND, int WM, int WN, int MI, int NI, bool LORA>
+__global__ __launch_bounds__(64 * WM * WN) void k_linear_gemm(LinearArgs p, int tm, int tn) {
+  constexpr int NW = WM * WN, BM = 16 * WM * MI, BN = 16 * WN * NI;
+  constexpr int BB = KIND == kBI ? 1024 : 2048;  // weight bytes of a column group per step
+  constexpr int SA = BM * 128, SB = BN / 16 * BB;
+  constexpr int AJ = BM / 8 / NW, BJ = SB / 1024 / NW;
+  static_assert(BM % (8 * NW) == 0 && SB % (1024 * NW) == 0 && BN / 16 % NW == 0, "whole loads per wave");
+  constexpr int kOrder = KIND == kII ? 0 : 1;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * (SA + SB)];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, q = lane >> 4;
+  const int wm = wv / WN, wn = wv % WN;
+  const int ntiles = tm * tn, per = (ntiles + 7) >> 3;
+  const int L = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || L >= ntiles) return;
+  constexpr int GM = 8;
+  const int grp = L / (GM * tn), in = L - grp * GM * tn, gsz = min(tm - grp * GM, GM);
+  const int mt = grp * GM + in % gsz, nt = in / gsz;
+  const int r0 = mt * BM, rows = min(BM, p.T - r0);
+  const int cg0 = nt * (BN / 16);
+  const uint32_t lds0 = lds_addr(smem);
+
+  uint32_t aoff[AJ];
+#pragma unroll
+  for (int j = 0; j < AJ; ++j) {
+    const int r = 8 * (wv + NW * j) + (lane >> 3);
+    const int pos = min(r0 + r, p.T - 1);
+    const int row = LORA ? p.order[pos] : pos;
+    aoff[j] = (uint32_t)row * p.row_bytes + (uint32_t)(a_piece_at<kOrder>(r, lane & 7) * 16);
+  }
+  const char* bsrc[BJ];
+#pragma unroll
+  for (int j = 0; j < BJ; ++j) {
+    const int at = (wv + NW * j) * 1024;
+    bsrc[j] = p.w + (size_t)min(cg0 + at / BB, p.cgs - 1) * p.cg_bytes + at % BB;
+  }
+  auto issue = [&](int s) {
+    const uint32_t st = lds0 + (uint32_t)((s & 1) * (SA + SB));
+#pragma unroll
+    for (int j = 0; j < AJ; ++j) dma16(aoff[j], p.x + (size_t)s * 128, st + (wv + NW * j) * 1024);
+#pragma unroll
+    for (int j = 0; j < BJ; ++j) dma16(lane * 16, bsrc[j] + (size_t)s * BB, st + SA + (wv + NW * j) * 1024);
+  };
+  floatx4 acc[MI][NI];
+  const int steps = KIND == kII ? (p.kc + 1) >> 1 : p.kc;
+  {
+    int32x4 iacc[KIND == kII ? MI : 1][KIND == kII ? NI : 1];
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (KIND == kII) iacc[m][n] = int32x4{0, 0, 0, 0};
+      }
+    issue(0);
+    vm_barrier<0>();
+    for (int s = 0; s < steps; ++s) {
+      if (s + 1 < steps) issue(s + 1);
+      const uint16_t* As = reinterpret_cast<const uint16_t*>(smem + (s & 1) * (SA + SB)) + wm * MI * 16 * 64;
+      const uint8_t* Bs = smem + (s & 1) * (SA + SB) + SA + wn * NI * BB + lane * 16;
+      bf16x8 wf[2][NI];
+      if constexpr (KIND == kBI) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n) cvt16(*reinterpret_cast<const uint4*>(Bs + n * BB), wf[0][n], wf[1][n]);
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        if constexpr (KIND != kBI) {
+#pragma unroll
+          for (int n = 0; n < NI; ++n) wf[st][n] = *reinterpret_cast<const bf16x8*>(Bs + n * BB + st * 1024);
+        }
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+          const int r = m * 16 + c;
+          if constexpr (KIND == kII) {
+            const int32x4 a = *reinterpret_cast<const int32x4*>(As + a_at<0>(r, 4 * st + q));
+#pragma unroll
+            for (int n = 0; n < NI; ++n)
+              iacc[m][n] =
+                  __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int32x4, wf[st][n]), a, iacc[m][n], 0, 0, 0);
+          } else {
+            const bf16x8 a = *reinterpret_cast<const bf16x8*>(As + a_at<1>(r, 2 * q + st));
+#pragma unroll
+            for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(wf[st][n], a, acc[m][n]);
+          }
+        }
+      }
+      vm_barrier<0>();
+    }
+    // scaled to f32
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      float xs = 1.0f;
+      if constexpr (KIND == kII) {
+        const int pos = min(r0 + (wm * MI + m) * 16 + c, p.T - 1);
+        xs = p.xs[LORA ? p.order[pos] : pos];
+      }
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        const int cg = min(cg0 + wn * NI + n, p.cgs - 1);
+        if constexpr (KIND == kII) {
+          const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + cg * 16 + 4 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[m][n][j] = (float)iacc[m][n][j] * xs * sc[j];
+        } else if constexpr (KIND == kBI) {
+          const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + cg * 16 + 4 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[m][n][j] *= sc[j];
+        }
+      }
+    }
+  }
+  if constexpr (LORA) {
+    constexpr int LB = BN / 16 / NW;  // B loads per wave and step
+    const int rb = p.rp >> 5;
+    uint32_t uoff[AJ];
+#pragma unroll
+    for (int j = 0; j < AJ; ++j) {
+      const int r = 8 * (wv + NW * j) + (lane >> 3);
+      uoff[j] = (uint32_t)(min(r0 + r, p.T - 1) - r0) * (uint32_t)(rb * 128) +
+                (uint32_t)(a_piece_at<1>(r, lane & 7) * 16);
+    }
+    const char* ubase = reinterpret_cast<const char*>(p.u) + (size_t)r0 * rb * 128;
+    const int w0 = wm * MI * 16;  // the wave's rows in the tile
+    for (int pos = r0; pos < r0 + rows;) {
+      const int ad = __builtin_amdgcn_readfirstlane(p.sorted[pos]);
+      if (ad < 0) break;
+      const int end = min(max(__builtin_amdgcn_readfirstlane(p.offsets[ad + 1]), pos + 1), r0 + rows);
+      const int lo = pos - r0, hi = end - r0;  // the adapter's rows in the tile
+      for (int s = 0; s < rb; ++s) {
+#pragma unroll
+        for (int j = 0; j < AJ; ++j) dma16(uoff[j], ubase + s * 128, lds0 + (wv + NW * j) * 1024);
+#pragma unroll
+        for (int j = 0; j < LB; ++j) {
+          const int cg = min(cg0 + wv + NW * j, p.cgs - 1);
+          dma16(lane * 16, p.b + (((size_t)ad * p.cgs + cg) * rb + s) * 1024, lds0 + SA + (wv + NW * j) * 1024);
+        }
+        vm_barrier<0>();
+        const uint16_t* As = reinterpret_cast<const uint16_t*>(smem) + w0 * 64;
+        const uint8_t* Bs = smem + SA + wn * NI * 1024 + c * 16;
+        bf16x8 wf[2][NI];
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int n = 0; n < NI; ++n)
+            wf[st][n] = *reinterpret_cast<const bf16x8*>(Bs + n * 1024 + (2 * (q & 1) + st) * 256);
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+          const int g0 = w0 + m * 16;
+          if (g0 + 16 <= lo || g0 >= hi) continue;
+          const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(As + a_at<1>(m * 16 + c, 2 * q));
+          const bf16x8 a1 = *reinterpret_cast<const bf16x8*>(As + a_at<1>(m * 16 + c, 2 * q + 1));
+          if (g0 >= lo && g0 + 16 <= hi) {
+#pragma unroll
+            for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, acc[m][n]));
+          } else {
+            const bool mine = g0 + c >= lo && g0 + c < hi;
+#pragma unroll
+            for (int n = 0; n < NI; ++n) {
+              const floatx4 t = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, floatx4{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[m][n][j] = mine ? acc[m][n][j] + t[j] : acc[m][n][j];
+            }
+          }
+        }
+        vm_barrier<0>();
+      }
+      pos = end;
+    }
+  }
+  const bool vec = (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+    const int pos = r0 + (wm * MI + m) * 16 + c;
+    if (pos >= p.T) continue;
+    uint16_t* o = p.out + (size_t)(LORA ? p.order[pos] : pos) * p.N;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int cg = cg0 + wn * NI + n;
+      if (cg >= p.cgs) continue;
+      const float v[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
+      store4(o, cg * 16 + 4 * q, p.N, vec, v);
+    }
+  }
+}
+
+}  // namespace kmoe
+
+namespace kmoe_host {
+
+using namespace kmoe;
+
+namespace {
+
+dim3 grid_for(int64_t items) {
+  const int64_t blocks = (items + 255) / 256;
+  return dim3((unsigned)(blocks < 1 ? 1 : (blocks > 65536 ? 65536 : blocks)));
+}
+
+template <int KIND, int RB>
+void decode_of(const LinearArgs& p, hipStream_t st) {
+  hipLaunchKernelGGL((k_linear_decode<KIND, RB, 2>), dim3((p.cgs + 1) / 2), dim3(512), 0, st, p);
+}
+
+template <int KIND>
+void decode(const LinearArgs& p, hipStream_t st) {
+  switch ((p.T + 15) / 16) {
+    case 1:
+      return decode_of<KIND, 1>(p, st);
+    case 2:
+      return decode_of<KIND, 2>(p, st);
+    case 3:
+      return decode_of<KIND, 3>(p, st);
+    default:
+      return decode_of<KIND, 4>(p, st);
+  }
+}
+
+template <int KIND, int WM, int WN, int MI, int NI>
+void gemm_of(const LinearArgs& p, hipStream_t st) {
+  constexpr int BM = 16 * WM * MI, BN = 16 * WN * NI;
+  const int tm = (p.T + BM - 1) / BM, tn = (p.cgs * 16 + BN - 1) / BN;
+  const dim3 grid((unsigned)((((int64_t)tm * tn + 7) >> 3) * 8));
+  if (p.adapter)
+    hipLaunchKernelGGL((k_linear_gemm<KIND, WM, WN, MI, NI, true>), grid, dim3(64 * WM * WN), 0, st, p, tm, tn);
+  else
+    hipLaunchKernelGGL((k_linear_gemm<KIND, WM, WN, MI, NI, false>), grid, dim3(64 * WM * WN), 0, st, p, tm, tn);
+}
+
+template <int KIND>
+void linear_kind(const LinearArgs& p, hipStream_t st) {
+  if (p.T <= kLinearDecodeTokens) {
+    if (p.adapter)
+      hipLaunchKernelGGL((k_lora_shrink_rows<KIND>), dim3(p.T, (p.rank + 15) / 16), dim3(1024), 0, st, p);
+    decode<KIND>(p, st);
+    return;
+  }
+  if (p.adapter) hipLaunchKernelGGL((k_lora_shrink<KIND>), dim3((p.T + 15) / 16), dim3(512), 0, st, p);
+  gemm_of<KIND, 2, 2, 4, 4>(p, st);
+}
+
+}  // namespace
+
+hipError_t launch_linear_pack(const kmoe_weight& w, const kmoe_linear_weight& packed, hipStream_t st) {
+  const int K = (int)packed.in_features, N = (int)packed.out_features;
+  const int Kp = (int)padded_in(K), Np = (int)padded_out(N);
+  if (packed.dtype == KMOE_DTYPE_BF16)
+    hipLaunchKernelGGL(k_pack_bf16, grid_for((int64_t)Kp * Np / 8), dim3(256), 0, st, (int64_t)1, K, N, Kp, Np,
+                       reinterpret_cast<const uint16_t*>(w.values), reinterpret_cast<uint16_t*>(packed.values));
+  else
+    hipLaunchKernelGGL(k_pack_i8, grid_for((int64_t)Kp * Np / 16), dim3(256), 0, st, K, N, Kp, Np,
+                       reinterpret_cast<const uint8_t*>(w.values), reinterpret_cast<uint8_t*>(packed.values));
+  hipLaunchKernelGGL(k_pack_scale, dim3((Np + 255) / 256), dim3(256), 0, st, N, Np, (int)w.scale_kind,
+                     w.scale_dtype == KMOE_DTYPE_BF16 ? 1 : 0, w.scale, packed.scale);
+  return hipGetLastError();
+}
+
+hipError_t launch_lora_pack(const kmoe_lora& l, int64_t first, int64_t count, int64_t rank, const void* a,
+                            const void* b, const float* factor, hipStream_t st) {
+  const int K = (int)l.in_features, N = (int)l.out_features, rp = (int)padded_rank(l.rank);
+  const int Kp = (int)padded_in(K), Np = (int)padded_out(N);
+  hipLaunchKernelGGL(k_pack_bf16, grid_for(count * rp * Kp / 8), dim3(256), 0, st, count, K, (int)rank, Kp, rp,
+                     reinterpret_cast<const uint16_t*>(a), reinterpret_cast<uint16_t*>(l.a) + (size_t)first * rp * Kp);
+  hipLaunchKernelGGL(k_pack_lora_b, grid_for(count * rp * Np / 8), dim3(256), 0, st, count, (int)rank, N, rp, Np,
+                     reinterpret_cast<const uint16_t*>(b), reinterpret_cast<uint16_t*>(l.b) + (size_t)first * rp * Np);
+  hipLaunchKernelGGL(k_copy_f32, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, count, factor,
+                     l.factor + first);
+  return hipGetLastError();
+}
+
+hipError_t launch_lora_sort(const int32_t* adapter, const kmoe_lora_batch& b, void* scratch, hipStream_t st) {
+  const int T = (int)b.tokens, L = (int)b.num_adapters, blocks = (T + kLoraSortBlock - 1) / kLoraSortBlock;
+  int32_t* hist = reinterpret_cast<int32_t*>(scratch);
+  if (blocks > 1)
+    hipLaunchKernelGGL(k_lora_count, dim3(blocks), dim3(kLoraSortBlock), 0, st, T, L, adapter, hist);
+  hipLaunchKernelGGL(k_lora_sort, dim3(blocks), dim3(kLoraSortBlock), 0, st, T, L, adapter, hist, blocks, b.adapter,
+                     b.order, b.sorted, b.offsets);
+  return hipGetLastError();
+}
+
+hipError_t launch_linear(const kmoe_linear_weight& w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                         int64_t x_stride, const float* x_scale, const kmoe_lora* lora, const kmoe_lora_batch* batch,
+                         void* out, void* workspace, const LinearSpace& space, hipStream_t st) {
+  const int K = (int)w.in_features, Kp = (int)padded_in(K);
+  const size_t size = dtype_size(x_dtype);
+  char* const ws = reinterpret_cast<char*>(workspace);
+  LinearArgs p{};
+  p.x = reinterpret_cast<const char*>(x);
+  p.row_bytes = (uint32_t)(x_stride * (int64_t)size);
+  if (!linear_rows_fit(w, x, x_dtype, x_stride)) {
+    const dim3 grid = grid_for(tokens * Kp);
+    if (x_dtype == KMOE_DTYPE_I8)
+      hipLaunchKernelGGL((k_stage_rows<uint8_t>), grid, dim3(256), 0, st, tokens, K, Kp, x_stride,
+                         reinterpret_cast<const uint8_t*>(x), reinterpret_cast<uint8_t*>(ws));
+    else
+      hipLaunchKernelGGL((k_stage_rows<uint16_t>), grid, dim3(256), 0, st, tokens, K, Kp, x_stride,
+                         reinterpret_cast<const uint16_t*>(x), reinterpret_cast<uint16_t*>(ws));
+    p.x = ws;
+    p.row_bytes = (uint32_t)(Kp * size);
+  }
+  p.xs = x_scale;
+  p.w = reinterpret_cast<const char*>(w.values);
+  p.ws = w.scale;
+  p.out = reinterpret_cast<uint16_t*>(out);
+  p.T = (int)tokens;
+  p.N = (int)w.out_features;
+  p.kc = (K + 63) / 64;
+  p.cgs = (int)(padded_out(w.out_features) / 16);
+  p.cg_bytes = (size_t)Kp * 16 * dtype_size(w.dtype);
+  if (lora) {
+    p.adapter = batch->adapter;
+    p.order = batch->order;
+    p.sorted = batch->sorted;
+    p.offsets = batch->offsets;
+    p.a = reinterpret_cast<const char*>(lora->a);
+    p.b = reinterpret_cast<const char*>(lora->b);
+    p.factor = lora->factor;
+    p.rank = (int)lora->rank;
+    p.rp = (int)padded_rank(lora->rank);
+    p.kcp = Kp / 64;
+    p.u = ws + space.u;
+  }
+  if (x_dtype == KMOE_DTYPE_I8)
+    linear_kind<kII>(p, st);
+  else if (w.dtype == KMOE_DTYPE_I8)
+    linear_kind<kBI>(p, st);
+  else
+    linear_kind<kBB>(p, st);
+  return hipGetLastError();
+}
+
+}  // namespace kmoe_host

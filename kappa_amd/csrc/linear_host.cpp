@@ -1,0 +1,218 @@
+// Host-only side of the projections and their adapters (see linear.h). No HIP call
+// is made here; the entry points in linear_api.hip run these checks first.
+#include "linear.h"
+
+namespace kmoe_host {
+
+namespace {
+
+constexpr int64_t kMostIn = (int64_t)1 << 16;  // int8 sums stay inside i32
+constexpr int64_t kMostOut = (int64_t)1 << 20;
+constexpr int64_t kMostTokens = (int64_t)1 << 24;
+constexpr int64_t kMostRowBytes = (int64_t)1 << 32;  // 32-bit load offsets
+
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+kmoe_status check_tokens(int64_t tokens) {
+  if (tokens < 0) return fail(KMOE_ERR_INVALID_ARG, "tokens must be >= 0 (got %lld)", (long long)tokens);
+  if (tokens > kMostTokens) return fail(KMOE_ERR_UNSUPPORTED, "tokens %lld too large", (long long)tokens);
+  return KMOE_OK;
+}
+
+kmoe_status check_x_dtype(const kmoe_linear_weight& w, kmoe_dtype x_dtype) {
+  const int x = enum_value(x_dtype);
+  if (x != KMOE_DTYPE_BF16 && x != KMOE_DTYPE_I8)
+    return fail(KMOE_ERR_INVALID_ARG, "x must be BF16 or I8 rows");
+  if (x == KMOE_DTYPE_I8 && enum_value(w.dtype) != KMOE_DTYPE_I8)
+    return fail(KMOE_ERR_INVALID_ARG, "8-bit rows need int8 weights");
+  return KMOE_OK;
+}
+
+kmoe_status check_beside(const kmoe_linear_weight& w, const kmoe_lora& l) {
+  if (l.in_features != w.in_features || l.out_features != w.out_features)
+    return fail(KMOE_ERR_INVALID_ARG, "the adapters are [%lld, %lld], the weights [%lld, %lld]",
+                (long long)l.in_features, (long long)l.out_features, (long long)w.in_features,
+                (long long)w.out_features);
+  return KMOE_OK;
+}
+
+}  // namespace
+
+bool linear_rows_fit(const kmoe_linear_weight& w, const void* x, kmoe_dtype x_dtype, int64_t x_stride) {
+  return w.in_features % step_of(x_dtype) == 0 && aligned16(x) &&
+         x_stride * (int64_t)dtype_size(x_dtype) % 16 == 0;
+}
+
+LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora) {
+  LinearSpace s;
+  s.u = align256((size_t)tokens * (size_t)padded_in(w.in_features) * dtype_size(x_dtype));
+  // f32 per token and rank, or two bf16
+  s.total = s.u + (lora ? align256((size_t)tokens * (size_t)padded_rank(lora->rank) * 4) : 0);
+  return s;
+}
+
+kmoe_status check_linear_weight(const kmoe_linear_weight* w, bool buffers) {
+  if (!w) return fail(KMOE_ERR_INVALID_ARG, "the packed weights are NULL");
+  const int t = enum_value(w->dtype);
+  if (t != KMOE_DTYPE_BF16 && t != KMOE_DTYPE_I8)
+    return fail(KMOE_ERR_INVALID_ARG, "packed weights are BF16 or I8");
+  if (w->in_features < 1 || w->out_features < 1)
+    return fail(KMOE_ERR_INVALID_ARG, "in_features and out_features must be >= 1");
+  if (w->in_features > kMostIn || w->out_features > kMostOut)
+    return fail(KMOE_ERR_UNSUPPORTED, "weights [%lld, %lld] too large", (long long)w->in_features,
+                (long long)w->out_features);
+  if (buffers && (!w->values || !w->scale))
+    return fail(KMOE_ERR_INVALID_ARG, "packed weights: every buffer must be non-NULL");
+  if (buffers && (!aligned16(w->values) || !aligned16(w->scale)))
+    return fail(KMOE_ERR_INVALID_ARG, "packed weights: the buffers must be 16-byte aligned");
+  return KMOE_OK;
+}
+
+kmoe_status check_lora(const kmoe_lora* l, bool buffers) {
+  if (!l) return fail(KMOE_ERR_INVALID_ARG, "lora is NULL");
+  if (l->num_adapters < 1 || l->rank < 1 || l->in_features < 1 || l->out_features < 1)
+    return fail(KMOE_ERR_INVALID_ARG, "num_adapters, rank, in_features and out_features must be >= 1");
+  if (l->num_adapters > kmoe::kLoraMaxAdapters)
+    return fail(KMOE_ERR_UNSUPPORTED, "num_adapters %lld exceeds %d", (long long)l->num_adapters,
+                kmoe::kLoraMaxAdapters);
+  if (l->rank > kmoe::kLoraMaxRank)
+    return fail(KMOE_ERR_UNSUPPORTED, "rank %lld exceeds %d", (long long)l->rank, kmoe::kLoraMaxRank);
+  if (l->in_features > kMostIn || l->out_features > kMostOut)
+    return fail(KMOE_ERR_UNSUPPORTED, "adapters [%lld, %lld] too large", (long long)l->in_features,
+                (long long)l->out_features);
+  if (buffers && (!l->a || !l->b || !l->factor))
+    return fail(KMOE_ERR_INVALID_ARG, "adapters: every buffer must be non-NULL");
+  if (buffers && (!aligned16(l->a) || !aligned16(l->b)))
+    return fail(KMOE_ERR_INVALID_ARG, "adapters: the buffers must be 16-byte aligned");
+  return KMOE_OK;
+}
+
+kmoe_status validate_linear_pack_bytes(const kmoe_linear_weight* p, size_t* values, size_t* scale) {
+  KMOE_TRY(check_linear_weight(p, false));
+  if (!values || !scale) return fail(KMOE_ERR_INVALID_ARG, "kmoe_linear_pack_bytes: NULL result");
+  const size_t out = (size_t)padded_out(p->out_features);
+  *values = (size_t)padded_in(p->in_features) * out * dtype_size(p->dtype);
+  *scale = 4 * out;
+  return KMOE_OK;
+}
+
+kmoe_status validate_linear_pack(const kmoe_weight* w, const kmoe_linear_weight* p) {
+  KMOE_TRY(check_weight(w, "the projection's"));
+  KMOE_TRY(check_linear_weight(p, true));
+  if (enum_value(w->dtype) != enum_value(p->dtype))
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_linear_pack: the weights are BF16 or I8, as the packed copy");
+  return KMOE_OK;
+}
+
+kmoe_status validate_lora_pack_bytes(const kmoe_lora* l, size_t* a, size_t* b) {
+  KMOE_TRY(check_lora(l, false));
+  if (!a || !b) return fail(KMOE_ERR_INVALID_ARG, "kmoe_lora_pack_bytes: NULL result");
+  const size_t per = 2 * (size_t)padded_rank(l->rank) * (size_t)l->num_adapters;
+  *a = per * (size_t)padded_in(l->in_features);
+  *b = per * (size_t)padded_out(l->out_features);
+  return KMOE_OK;
+}
+
+kmoe_status validate_lora_pack(const kmoe_lora* l, int64_t first, int64_t count, int64_t rank, const void* a,
+                               const void* b, const float* factor) {
+  KMOE_TRY(check_lora(l, true));
+  if (first < 0 || count < 0 || first > l->num_adapters || count > l->num_adapters - first)
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_lora_pack: %lld slots from %lld on, of %lld", (long long)count,
+                (long long)first, (long long)l->num_adapters);
+  if (rank < 1 || rank > l->rank)
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_lora_pack: rank %lld is not in [1, %lld]", (long long)rank,
+                (long long)l->rank);
+  if (count > 0 && (!a || !b || !factor)) return fail(KMOE_ERR_INVALID_ARG, "kmoe_lora_pack: NULL buffer");
+  return KMOE_OK;
+}
+
+namespace {
+
+kmoe_status check_batch(const kmoe_lora_batch* b, bool buffers) {
+  if (!b) return fail(KMOE_ERR_INVALID_ARG, "batch is NULL");
+  KMOE_TRY(check_tokens(b->tokens));
+  if (b->num_adapters < 1) return fail(KMOE_ERR_INVALID_ARG, "num_adapters must be >= 1");
+  if (b->num_adapters > kmoe::kLoraMaxAdapters)
+    return fail(KMOE_ERR_UNSUPPORTED, "num_adapters %lld exceeds %d", (long long)b->num_adapters,
+                kmoe::kLoraMaxAdapters);
+  if (buffers && (!b->adapter || !b->order || !b->sorted || !b->offsets))
+    return fail(KMOE_ERR_INVALID_ARG, "batch: every buffer must be non-NULL");
+  return KMOE_OK;
+}
+
+size_t sort_bytes(const kmoe_lora_batch& b) {
+  const size_t blocks = ((size_t)b.tokens + kmoe::kLoraSortBlock - 1) / kmoe::kLoraSortBlock;
+  return 4 * blocks * (size_t)(b.num_adapters + 1);
+}
+
+}  // namespace
+
+kmoe_status validate_lora_sort_bytes(const kmoe_lora_batch* b, size_t* bytes) {
+  KMOE_TRY(check_batch(b, false));
+  if (!bytes) return fail(KMOE_ERR_INVALID_ARG, "bytes is NULL");
+  *bytes = sort_bytes(*b);
+  return KMOE_OK;
+}
+
+kmoe_status validate_lora_sort(const int32_t* adapter, const kmoe_lora_batch* b, const void* scratch,
+                               size_t scratch_bytes) {
+  KMOE_TRY(check_batch(b, true));
+  if (b->tokens > 0 && !adapter) return fail(KMOE_ERR_INVALID_ARG, "kmoe_lora_sort: NULL buffer");
+  if (b->tokens > 0 && (!scratch || scratch_bytes < sort_bytes(*b)))
+    return fail(KMOE_ERR_WORKSPACE_TOO_SMALL, "kmoe_lora_sort: scratch of %zu bytes is smaller than the %zu required",
+                scratch_bytes, sort_bytes(*b));
+  return KMOE_OK;
+}
+
+kmoe_status validate_linear_workspace_bytes(const kmoe_linear_weight* w, int64_t tokens, kmoe_dtype x_dtype,
+                                            const kmoe_lora* lora, size_t* bytes) {
+  KMOE_TRY(check_linear_weight(w, false));
+  KMOE_TRY(check_tokens(tokens));
+  KMOE_TRY(check_x_dtype(*w, x_dtype));
+  if (lora) {
+    KMOE_TRY(check_lora(lora, false));
+    KMOE_TRY(check_beside(*w, *lora));
+  }
+  if (!bytes) return fail(KMOE_ERR_INVALID_ARG, "bytes is NULL");
+  *bytes = linear_space(*w, tokens, x_dtype, lora).total;
+  return KMOE_OK;
+}
+
+kmoe_status validate_linear(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                            int64_t x_stride, const float* x_scale, const kmoe_lora* lora,
+                            const kmoe_lora_batch* batch, const void* out, const void* workspace,
+                            size_t workspace_bytes, LinearSpace* space) {
+  KMOE_TRY(check_linear_weight(w, true));
+  KMOE_TRY(check_tokens(tokens));
+  KMOE_TRY(check_x_dtype(*w, x_dtype));
+  if (x_stride < w->in_features && tokens > 0)
+    return fail(KMOE_ERR_INVALID_ARG, "x_stride %lld is smaller than in_features %lld", (long long)x_stride,
+                (long long)w->in_features);
+  if ((enum_value(x_dtype) == KMOE_DTYPE_I8) != (x_scale != nullptr) && tokens > 0)
+    return fail(KMOE_ERR_INVALID_ARG, "x_scale comes with I8 rows, and with those only");
+  if (!lora != !batch) return fail(KMOE_ERR_INVALID_ARG, "lora and batch come together");
+  if (lora) {
+    KMOE_TRY(check_lora(lora, true));
+    KMOE_TRY(check_beside(*w, *lora));
+    KMOE_TRY(check_batch(batch, true));
+    if (batch->tokens != tokens || batch->num_adapters != lora->num_adapters)
+      return fail(KMOE_ERR_INVALID_ARG,
+                  "the batch holds %lld tokens of %lld adapters; the call has %lld tokens and %lld adapters",
+                  (long long)batch->tokens, (long long)batch->num_adapters, (long long)tokens,
+                  (long long)lora->num_adapters);
+  }
+  const int64_t size = (int64_t)dtype_size(x_dtype);
+  const int64_t row = (kMostRowBytes - 1) / (tokens > 0 ? tokens : 1);  // bytes of a row and what follows it
+  if (tokens > 0 && (x_stride > kMostRowBytes || x_stride * size > row || padded_in(w->in_features) * size > row))
+    return fail(KMOE_ERR_UNSUPPORTED, "x must span less than 4 GiB");
+  if (tokens > 0 && (!x || !out)) return fail(KMOE_ERR_INVALID_ARG, "kmoe_linear: x and out must be non-NULL");
+  *space = linear_space(*w, tokens, x_dtype, lora);
+  if (tokens > 0 && (!workspace || workspace_bytes < space->total))
+    return fail(KMOE_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes is smaller than the %zu required",
+                workspace_bytes, space->total);
+  if (tokens > 0 && !aligned16(workspace))
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_linear: the workspace must be 16-byte aligned");
+  return KMOE_OK;
+}
+
+}  // namespace kmoe_host

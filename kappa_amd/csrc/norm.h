@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.h"
+#include "expert_dev.h"
 
 namespace kmoe {
 
@@ -25,6 +26,13 @@ struct NormRow {
   __device__ __forceinline__ static bool pieces(const A* src, int D) {
     return D % kRouterSlice == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
   }
+  // the inverse of unpack, rounding to A
+  __device__ __forceinline__ static uint4 pack(const float* f) {
+    if constexpr (sizeof(A) == 2)
+      return uint4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+    else
+      return uint4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+  }
   __device__ __forceinline__ static void unpack(const uint4& v, float* f) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -39,23 +47,60 @@ struct NormRow {
   }
 };
 
-// One wave: stage the row src[0..D) in LDS (NormRow) and return
-//   r = 1 / sqrt(S / D + eps),  S = sum_d src[d]^2
-// in the canonical order: each square rounded to float, lane s adds the
-// squares of slice s (64 indices) in a sequential chain from +0.0f, and the
-// slice sums are combined by the zero-padded pairwise tree p[l] += p[l + st]
-// (the router's order); IEEE division and square root. The row stays in LDS
-// for the caller and, where it moves in pieces (NormRow::pieces), piece lane + 64 i
-// in v[i]; every lane of the wave must call it, and gets r.
+// One wave: r = 1 / sqrt(S / D + eps), S = sum_d row[d]^2, of a row that the wave has
+// staged in LDS (NormRow, the last slice filled up with zeros), in the canonical order:
+// each square rounded to float, lane s adds the squares of slice s (64 indices) in a
+// sequential chain from +0.0f, and the slice sums are combined by the zero-padded
+// pairwise tree p[l] += p[l + st] (the router's order); IEEE division and square
+// root. Every lane of the wave must call it, and gets r.
 template <typename A>
-__device__ __forceinline__ float wave_rms_factor(const A* __restrict__ src, int D, float eps, A* row,
-                                                 uint4 (&v)[NormRow<A>::kPieces]) {
+__device__ __forceinline__ float wave_rms_reduce(const A* row, int D, float eps) {
 #pragma clang fp contract(off)
   using R = NormRow<A>;
   const int lane = threadIdx.x & 63;
   const int NS = (D + kRouterSlice - 1) / kRouterSlice;
   int P = 1;
   while (P < NS) P <<= 1;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  float acc = 0.0f;
+  if (lane < NS) {
+    const A* sl = row + lane * R::kSlice;
+    // the slice's reads are all in flight before the chain starts
+    uint4 p[kRouterSlice / R::kPiece];
+#pragma unroll
+    for (int i = 0; i < kRouterSlice / R::kPiece; ++i) p[i] = reinterpret_cast<const uint4*>(sl)[i];
+#pragma unroll
+    for (int i = 0; i < kRouterSlice / R::kPiece; ++i) {
+      float f[R::kPiece];
+      R::unpack(p[i], f);
+#pragma unroll
+      for (int j = 0; j < R::kPiece; ++j) {
+        const float sq = f[j] * f[j];
+        acc = acc + sq;
+      }
+    }
+  }
+  for (int st = 1; st < P; st <<= 1) {
+    const float o = __shfl_down(acc, st, 64);
+    if ((lane & (2 * st - 1)) == 0) acc = acc + o;
+  }
+  const float total = __shfl(acc, 0, 64);
+  const float var = total / (float)D;
+  return 1.0f / sqrtf(var + eps);
+}
+
+// One wave: stage the row src[0..D) in LDS (NormRow) and return its factor r
+// (wave_rms_reduce). The row stays in LDS for the caller and, where it moves in pieces
+// (NormRow::pieces), piece lane + 64 i in v[i]; every lane of the wave must call it, and
+// gets r.
+template <typename A>
+__device__ __forceinline__ float wave_rms_factor(const A* __restrict__ src, int D, float eps, A* row,
+                                                 uint4 (&v)[NormRow<A>::kPieces]) {
+  using R = NormRow<A>;
+  const int lane = threadIdx.x & 63;
+  const int NS = (D + kRouterSlice - 1) / kRouterSlice;
   const bool pieces = R::pieces(src, D);
   if (pieces) {
     const int n = D / R::kPiece;
@@ -89,34 +134,7 @@ __device__ __forceinline__ float wave_rms_factor(const A* __restrict__ src, int 
     const int tail = (NS - 1) * kRouterSlice + lane;
     if (tail >= D) row[R::at(tail)] = 0;
   }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  float acc = 0.0f;
-  if (lane < NS) {
-    const A* sl = row + lane * R::kSlice;
-    // the slice's reads are all in flight before the chain starts
-    uint4 p[kRouterSlice / R::kPiece];
-#pragma unroll
-    for (int i = 0; i < kRouterSlice / R::kPiece; ++i) p[i] = reinterpret_cast<const uint4*>(sl)[i];
-#pragma unroll
-    for (int i = 0; i < kRouterSlice / R::kPiece; ++i) {
-      float f[R::kPiece];
-      R::unpack(p[i], f);
-#pragma unroll
-      for (int j = 0; j < R::kPiece; ++j) {
-        const float sq = f[j] * f[j];
-        acc = acc + sq;
-      }
-    }
-  }
-  for (int st = 1; st < P; st <<= 1) {
-    const float o = __shfl_down(acc, st, 64);
-    if ((lane & (2 * st - 1)) == 0) acc = acc + o;
-  }
-  const float total = __shfl(acc, 0, 64);
-  const float var = total / (float)D;
-  return 1.0f / sqrtf(var + eps);
+  return wave_rms_reduce(row, D, eps);
 }
 
 // One normalised element: round_act((x * r) * scale), each product rounded.

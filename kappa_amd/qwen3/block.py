@@ -19,6 +19,7 @@ import torch
 from .. import _lib
 from .architecture import Qwen3Config
 from .ffn_moe import PackedExperts, _desc, _impl_and_capacity, _moe_forward, _norm_scale, _stream
+from .projection import Q8Rows, _OnDevice
 from .quant import Weight, kmoe_dtype
 
 
@@ -46,6 +47,70 @@ def rms_norm(
         )
     )
     return out.reshape(x.shape)
+
+
+def _norm_inputs(x: torch.Tensor, residual: torch.Tensor | None, scale: torch.Tensor):
+    """Flattened contiguous x and residual, the norm scale, T and D."""
+    if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
+        raise ValueError(f"x must be a torch tensor on a HIP device (got {getattr(x, 'device', type(x))})")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"x must be bfloat16 or float32 (got {x.dtype})")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one axis")
+    if residual is not None and (
+        not isinstance(residual, torch.Tensor)
+        or residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device
+    ):  # fmt: skip
+        raise ValueError(
+            f"residual must be as x, {tuple(x.shape)} {x.dtype} on {x.device} (got "
+            f"{tuple(getattr(residual, 'shape', ()))} {getattr(residual, 'dtype', type(residual))} on "
+            f"{getattr(residual, 'device', None)})"
+        )
+    d = int(x.shape[-1])
+    sc = _norm_scale(scale, d, x.device)
+    return x.contiguous(), None if residual is None else residual.contiguous(), sc, x.numel() // d if d else 0, d
+
+
+def add_rms_norm(
+    x: torch.Tensor, residual: torch.Tensor, scale: torch.Tensor, *, epsilon: float = 1e-6
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The residual's addition and the norm after it, in one pass: ``(rms_norm(h, scale), h)``
+    with ``h = x + residual`` (kappa/qwen3/block.py:71, 153, 196), bit for bit what the two
+    steps give. ``x`` and ``residual`` are ``[..., D]`` of one type, bfloat16 or float32."""
+    x, residual, sc, T, d = _norm_inputs(x, residual, scale)
+    if residual is None:
+        raise ValueError("add_rms_norm needs a residual (rms_norm takes none)")
+    with _OnDevice(x.device):
+        h, out = torch.empty_like(x), torch.empty_like(x)
+        _lib.check(
+            _lib.lib().kmoe_add_rms_norm(
+                _desc(T, d, 1, 1, 1, x.dtype), x.data_ptr(), residual.data_ptr(), sc.data_ptr(), kmoe_dtype(sc.dtype),
+                float(epsilon), h.data_ptr(), out.data_ptr(), _stream(x.device),
+            )
+        )  # fmt: skip
+    return out, h
+
+
+def add_rms_norm_q8(
+    x: torch.Tensor, residual: torch.Tensor | None, scale: torch.Tensor, *, epsilon: float = 1e-6
+) -> tuple[Q8Rows, torch.Tensor]:
+    """``add_rms_norm`` with the normalised rows in 8 bits, for ``linear``: ``(rows, h)``. With
+    ``v`` the normalised row in float32, ``rows.scale = max|v| / 127`` and ``rows.values =
+    rint(v / rows.scale)``; a row with an infinity or a NaN has a NaN scale. ``residual`` may
+    be None (``h`` is ``x``)."""
+    x, residual, sc, T, d = _norm_inputs(x, residual, scale)
+    with _OnDevice(x.device):
+        h = x if residual is None else torch.empty_like(x)
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        s = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+        _lib.check(
+            _lib.lib().kmoe_add_rms_norm_q8(
+                _desc(T, d, 1, 1, 1, x.dtype), x.data_ptr(), None if residual is None else residual.data_ptr(),
+                sc.data_ptr(), kmoe_dtype(sc.dtype), float(epsilon), None if residual is None else h.data_ptr(),
+                q.data_ptr(), s.data_ptr(), _stream(x.device),
+            )
+        )  # fmt: skip
+    return Q8Rows(q, s), h
 
 
 def moe_block_ffn(

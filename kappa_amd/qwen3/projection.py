@@ -1,0 +1,273 @@
+"""Projections of a decoder layer on MI355X, and the low-rank adapters of many requests
+beside them.
+
+``linear(x, w)`` is the ``x @ to_compute_dtype(w)`` of the reference's q, k, v and o
+projections (kappa/qwen3/linear.py:10-25) with the heads side by side in the last axis. ``w`` is laid out
+once by ``prepack_linear`` (bf16, or a ``Q8Weight`` whose scale multiplies the f32 sum);
+``x`` is bf16 or the 8-bit rows of ``add_rms_norm_q8``.
+
+Adapters (the reference has none): ``prepack_lora`` lays out the adapters of one projection,
+``lora_batch`` sorts a step's tokens by adapter once, and every projection of the step takes
+that batch::
+
+    batch = lora_batch(adapter, num_adapters)          # adapter[t]: of token t, -1 for none
+    qkv = linear(normed, w_qkv, lora=lora_qkv, batch=batch)
+
+adds ``factor[a] * (x[t] @ a[a]) @ b[a]`` to token t's row. Like the rest of the package this
+is for inference: no gradients.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import NamedTuple, Union
+
+import torch
+
+from .. import _lib
+from .quant import Q8Weight, _require_cuda, is_q8_weight, weight_struct
+
+
+class Q8Rows(NamedTuple):
+    """Rows in int8 with one scale each: row ``t`` stands for ``values[t] * scale[t]``."""
+
+    values: torch.Tensor  # [..., D] int8
+    scale: torch.Tensor  # [..., 1] float32
+
+
+class _OnDevice:
+    """Makes a tensor's device the current one where it is not (launches go to the current device)."""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.index is not None and self.index != self.before:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index is not None and self.index != self.before:
+            torch.cuda.set_device(self.before)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+@dataclass(frozen=True)
+class PackedLinear:
+    """A projection's weights in the gfx950 layout (include/kmoe.h, kmoe_linear_weight)."""
+
+    values: torch.Tensor
+    scale: torch.Tensor
+    in_features: int
+    out_features: int
+    struct: _lib.KmoeLinear
+
+    @property
+    def nbytes(self) -> int:
+        return self.values.numel() * self.values.element_size() + 4 * self.scale.numel()
+
+
+def prepack_linear(w: Union[torch.Tensor, Q8Weight]) -> PackedLinear:
+    """One-time relayout of a projection's ``[in, out]`` weights for the MFMA kernels: bf16,
+    or a ``Q8Weight`` with one scale or one per output channel (``[out]`` or ``[1, out]``).
+    The copy holds the same values and does not follow later writes to ``w``."""
+    v = w.values if is_q8_weight(w) else w
+    _require_cuda(v, "w")
+    if v.dim() != 2:
+        raise ValueError(f"w must be [in, out] (got shape {tuple(v.shape)})")
+    if not is_q8_weight(w) and v.dtype != torch.bfloat16:
+        raise ValueError(f"w must be bfloat16 or a Q8Weight (got {v.dtype})")
+    K, N = (int(s) for s in v.shape)
+    dtype = torch.int8 if is_q8_weight(w) else torch.bfloat16
+    code = _lib.DTYPE_I8 if is_q8_weight(w) else _lib.DTYPE_BF16
+    st = _lib.KmoeLinear(None, None, code, K, N)
+    nv, ns = ctypes.c_size_t(), ctypes.c_size_t()
+    L = _lib.lib()
+    _lib.check(L.kmoe_linear_pack_bytes(st, ctypes.byref(nv), ctypes.byref(ns)))
+    with _OnDevice(v.device):
+        src, keep = weight_struct(w, v.device, n_out=N, n_groups=None, name="w")
+        values = torch.empty(nv.value // dtype.itemsize, dtype=dtype, device=v.device)
+        scale = torch.empty(ns.value // 4, dtype=torch.float32, device=v.device)
+        st.values, st.scale = values.data_ptr(), scale.data_ptr()
+        _lib.check(L.kmoe_linear_pack(src, st, _stream(v.device)))
+    return PackedLinear(values, scale, K, N, st)
+
+
+@dataclass(frozen=True)
+class LoraAdapters:
+    """The adapters of one projection in the gfx950 layout (include/kmoe.h, kmoe_lora)."""
+
+    a: torch.Tensor
+    b: torch.Tensor
+    factor: torch.Tensor
+    num_adapters: int
+    rank: int
+    in_features: int
+    out_features: int
+    struct: _lib.KmoeLora
+
+    @staticmethod
+    def empty(
+        num_adapters: int, rank: int, in_features: int, out_features: int, *, device: Union[str, torch.device] = "cuda"
+    ) -> LoraAdapters:
+        """Slots that add nothing until ``store`` fills them; ``rank`` is the largest they take."""
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"the adapters must be on a HIP device (got {device})")
+        st = _lib.KmoeLora(None, None, None, num_adapters, rank, in_features, out_features)
+        na, nb = ctypes.c_size_t(), ctypes.c_size_t()
+        _lib.check(_lib.lib().kmoe_lora_pack_bytes(st, ctypes.byref(na), ctypes.byref(nb)))
+        a = torch.zeros(na.value // 2, dtype=torch.bfloat16, device=device)
+        b = torch.zeros(nb.value // 2, dtype=torch.bfloat16, device=device)
+        factor = torch.zeros(num_adapters, dtype=torch.float32, device=device)
+        st.a, st.b, st.factor = a.data_ptr(), b.data_ptr(), factor.data_ptr()
+        return LoraAdapters(a, b, factor, num_adapters, rank, in_features, out_features, st)
+
+    def store(self, first: int, a: torch.Tensor, b: torch.Tensor, factor: Union[float, torch.Tensor]) -> None:
+        """Fills the slots ``first ..`` from ``a`` ``[count, in, r]`` and ``b`` ``[count, r, out]``
+        (bf16, ``r <= rank``; without the first axis: one slot) and ``factor`` (a number, or
+        ``[count]``; an adapter's alpha / r)."""
+        if a.dim() == 2 and b.dim() == 2:
+            a, b = a.unsqueeze(0), b.unsqueeze(0)
+        dev = self.a.device
+        for name, t in (("a", a), ("b", b)):
+            if t.device != dev or t.dtype != torch.bfloat16:
+                raise ValueError(f"{name} must be bfloat16 on {dev} (got {t.dtype} on {t.device})")
+        if a.dim() != 3 or b.dim() != 3:
+            raise ValueError(f"a and b must be [count, in, r] and [count, r, out] (got {tuple(a.shape)}, {tuple(b.shape)})")
+        count, K, r = (int(s) for s in a.shape)
+        if K != self.in_features or tuple(b.shape) != (count, r, self.out_features):
+            raise ValueError(
+                f"a {tuple(a.shape)} and b {tuple(b.shape)} are not [count, {self.in_features}, r] and "
+                f"[count, r, {self.out_features}]"
+            )
+        if isinstance(factor, torch.Tensor):
+            if factor.numel() != count:
+                raise ValueError(f"factor has {factor.numel()} entries for {count} adapters")
+            f = factor.reshape(count).to(device=dev, dtype=torch.float32).contiguous()
+        else:
+            f = torch.full((count,), float(factor), dtype=torch.float32, device=dev)
+        a, b = a.contiguous(), b.contiguous()
+        with _OnDevice(dev):
+            _lib.check(
+                _lib.lib().kmoe_lora_pack(
+                    self.struct, first, count, r, a.data_ptr(), b.data_ptr(), f.data_ptr(), _stream(dev)
+                )
+            )
+
+
+def prepack_lora(a: torch.Tensor, b: torch.Tensor, factor: Union[float, torch.Tensor] = 1.0) -> LoraAdapters:
+    """One-time relayout of a projection's adapters: ``a`` ``[L, in, rank]`` and ``b``
+    ``[L, rank, out]`` in bf16 (adapters of smaller rank filled up with zeros, or
+    ``LoraAdapters.empty`` and ``store``), ``factor`` a number or ``[L]``."""
+    _require_cuda(a, "a")
+    _require_cuda(b, "b")
+    if a.dim() != 3 or b.dim() != 3:
+        raise ValueError(f"a and b must be [L, in, rank] and [L, rank, out] (got {tuple(a.shape)}, {tuple(b.shape)})")
+    L, K, r = (int(s) for s in a.shape)
+    out = LoraAdapters.empty(L, r, K, int(b.shape[2]), device=a.device)
+    out.store(0, a, b, factor)
+    return out
+
+
+@dataclass(frozen=True)
+class LoraBatch:
+    """A step's tokens sorted by adapter (include/kmoe.h, kmoe_lora_batch)."""
+
+    buffer: torch.Tensor
+    tokens: int
+    num_adapters: int
+    struct: _lib.KmoeLoraBatch
+
+
+def lora_batch(adapter: torch.Tensor, num_adapters: int) -> LoraBatch:
+    """Sorts the tokens by ``adapter`` (int32 or int64, one per token, on the device); a value
+    outside ``[0, num_adapters)`` means none. The batch holds a copy of ``adapter``."""
+    _require_cuda(adapter, "adapter")
+    if adapter.dtype == torch.int64:
+        adapter = adapter.clamp(-1, num_adapters).to(torch.int32)
+    if adapter.dtype != torch.int32:
+        raise ValueError(f"adapter must be int32 or int64 (got {adapter.dtype})")
+    adapter = adapter.reshape(-1).contiguous()
+    T, dev = adapter.numel(), adapter.device
+    st = _lib.KmoeLoraBatch(None, None, None, None, T, num_adapters)
+    L = _lib.lib()
+    n = ctypes.c_size_t()
+    _lib.check(L.kmoe_lora_sort_bytes(st, ctypes.byref(n)))
+    with _OnDevice(dev):
+        buf = torch.empty(3 * T + num_adapters + 1 + n.value // 4, dtype=torch.int32, device=dev)
+        p = buf.data_ptr()
+        st.adapter, st.order, st.sorted, st.offsets = p, p + 4 * T, p + 8 * T, p + 12 * T
+        _lib.check(L.kmoe_lora_sort(adapter.data_ptr(), st, p + 4 * (3 * T + num_adapters + 1), n.value, _stream(dev)))
+    return LoraBatch(buf, T, num_adapters, st)
+
+
+def linear(
+    x: Union[torch.Tensor, Q8Rows],
+    w: PackedLinear,
+    *,
+    lora: LoraAdapters | None = None,
+    batch: LoraBatch | None = None,
+) -> torch.Tensor:
+    """``x @ w`` with the adapters of each token's request: ``[..., in]`` -> bf16 ``[..., out]``.
+
+    ``x`` is bf16, or 8-bit rows (which need int8 weights). Sums are f32 (8-bit rows: exact),
+    rounded once at the end. A row does not depend on the other rows' adapters."""
+    if not isinstance(w, PackedLinear):
+        raise ValueError(f"w must be a PackedLinear from prepack_linear (got {type(w).__name__})")
+    K = w.in_features
+    xs = None
+    if isinstance(x, Q8Rows):
+        v, scale = x
+        code = _lib.DTYPE_I8
+        if v.dtype != torch.int8 or scale.dtype != torch.float32:
+            raise ValueError(f"8-bit rows are int8 with float32 scales (got {v.dtype}, {scale.dtype})")
+        if w.values.dtype != torch.int8:
+            raise ValueError("8-bit rows need int8 weights")
+    else:
+        v, code = x, _lib.DTYPE_BF16
+        if not isinstance(v, torch.Tensor) or v.dtype != torch.bfloat16:
+            raise ValueError(f"x must be bfloat16 or Q8Rows (got {getattr(v, 'dtype', type(v).__name__)})")
+    dev = w.values.device
+    if v.device != dev:
+        raise ValueError(f"x is on {v.device}, w on {dev}")
+    if v.dim() < 1 or v.shape[-1] != K:
+        raise ValueError(f"x has shape {tuple(v.shape)}, the weights take rows of {K}")
+    shape = v.shape[:-1]
+    T = v.numel() // K
+    if code == _lib.DTYPE_I8:
+        if scale.device != dev or scale.numel() != T:
+            raise ValueError(f"the scales are {tuple(scale.shape)} on {scale.device}: one per row is wanted")
+        scale = scale.contiguous()
+        xs = scale.data_ptr()
+    # rows of one stride are read where they are
+    if not (v.dim() == 2 and v.stride(1) == 1 and v.stride(0) >= K):
+        v = v.reshape(T, K)
+        if v.stride(1) != 1 or v.stride(0) < K:
+            v = v.contiguous()
+    if (lora is None) != (batch is None):
+        raise ValueError("lora and batch come together")
+    ls = bs = None
+    if lora is not None:
+        if not isinstance(lora, LoraAdapters) or not isinstance(batch, LoraBatch):
+            raise ValueError("lora must be LoraAdapters from prepack_lora, batch a LoraBatch from lora_batch")
+        if lora.a.device != dev or batch.buffer.device != dev:
+            raise ValueError(f"the adapters are on {lora.a.device}, the batch on {batch.buffer.device}, w on {dev}")
+        ls, bs = lora.struct, batch.struct
+    L = _lib.lib()
+    n = ctypes.c_size_t()
+    _lib.check(L.kmoe_linear_workspace_bytes(w.struct, T, code, ls, ctypes.byref(n)))
+    with _OnDevice(dev):
+        out = torch.empty((*shape, w.out_features), dtype=torch.bfloat16, device=dev)
+        ws = torch.empty(max(n.value, 1), dtype=torch.uint8, device=dev)
+        _lib.check(
+            L.kmoe_linear(
+                w.struct, T, v.data_ptr(), code, v.stride(0) if T > 1 else K, xs, ls, bs, out.data_ptr(), ws.data_ptr(), n.value,
+                _stream(dev),
+            )
+        )  # fmt: skip
+    return out
