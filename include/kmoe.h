@@ -359,16 +359,20 @@ kmoe_status kmoe_lora_sort_bytes(const kmoe_lora_batch* batch, size_t* bytes);
 kmoe_status kmoe_lora_sort(const int32_t* adapter, const kmoe_lora_batch* batch, void* scratch, size_t scratch_bytes,
                            void* stream);
 
-/* Bytes of device workspace kmoe_linear needs for up to `tokens` rows of x_dtype (lora may be NULL). */
+/* Bytes of device workspace that serve every kmoe_linear of up to `tokens` rows of x_dtype
+ * (lora may be NULL), whatever the rows' stride and alignment. */
 kmoe_status kmoe_linear_workspace_bytes(const kmoe_linear_weight* w, int64_t tokens, kmoe_dtype x_dtype,
                                         const kmoe_lora* lora, size_t* bytes);
+/* What one call with these rows needs, which may be nothing: kmoe_linear takes no less. */
+kmoe_status kmoe_linear_call_bytes(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                                   int64_t x_stride, const kmoe_lora* lora, size_t* bytes);
 /* out[t] = round(x_scale[t] * w.scale * (x[t] @ w.values) [+ u[t] @ b[a]]),
  * u[t] = factor[a] * x_scale[t] * (x[t] @ a[a]) with a = batch->adapter[t] (nothing is added for -1).
  *   x       [T, in], rows x_stride elements apart: BF16 (x_scale NULL: 1), or I8 with
  *           x_scale [T] f32 (kmoe_add_rms_norm_q8's outputs), which takes I8 weights
  *   out     [T, out] BF16
  * Sums in f32 (int8 rows: exact in i32 first); u stays f32 up to 64 tokens and is carried as
- * bf16(u) + bf16(u - bf16(u)) above. lora and batch are both NULL or both given. x spans less than 4 GiB. */
+ * bf16(u) + bf16(u - bf16(u)) above. workspace may be NULL where kmoe_linear_call_bytes gives 0. lora and batch are both NULL or both given. x spans less than 4 GiB. */
 kmoe_status kmoe_linear(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
                         int64_t x_stride, const float* x_scale, const kmoe_lora* lora, const kmoe_lora_batch* batch,
                         void* out, void* workspace, size_t workspace_bytes, void* stream);

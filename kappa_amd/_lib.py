@@ -68,6 +68,7 @@ EXPORTS = (
     "kmoe_lora_sort_bytes",
     "kmoe_lora_sort",
     "kmoe_linear_workspace_bytes",
+    "kmoe_linear_call_bytes",
     "kmoe_linear",
     "kmoe_route",
     "kmoe_route_scratch_bytes",
@@ -234,6 +235,8 @@ def _declare(L: ctypes.CDLL) -> None:
     L.kmoe_lora_sort.argtypes = [_P, _BP, _P, ctypes.c_size_t, _P]
     L.kmoe_linear_workspace_bytes.restype = ctypes.c_int
     L.kmoe_linear_workspace_bytes.argtypes = [_LP, ctypes.c_int64, ctypes.c_int, _RP, _ZP]
+    L.kmoe_linear_call_bytes.restype = ctypes.c_int
+    L.kmoe_linear_call_bytes.argtypes = [_LP, ctypes.c_int64, _P, ctypes.c_int, ctypes.c_int64, _RP, _ZP]
     L.kmoe_linear.restype = ctypes.c_int
     L.kmoe_linear.argtypes = [
         _LP, ctypes.c_int64, _P, ctypes.c_int, ctypes.c_int64, _P, _RP, _BP, _P, _P, ctypes.c_size_t, _P,

@@ -19,6 +19,8 @@
 namespace kmoe {
 
 constexpr int kNormWaves = 4;  // tokens per block, one wave each
+constexpr int kNormNarrow = 128;    // 16-byte pieces of a row that one wave takes in add_rms_norm
+constexpr int kNormManyRows = 1000;  // above this many rows
 
 // 16 bytes (or the run of 16-byte loads) of the scale that go with a piece of the row
 template <typename A, typename S>
@@ -94,139 +96,181 @@ __global__ __launch_bounds__(256) void k_rms_norm(int T, int D, float eps, const
   }
 }
 
+namespace {
+
+// 16, 8 and 4 bytes at any element's address (the hardware takes dwords off their boundary)
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+
+__device__ __forceinline__ uint4 load16(const void* p) {
+  const u32x4_any v = *reinterpret_cast<const u32x4_any*>(p);
+  return uint4{v.x, v.y, v.z, v.w};
+}
+__device__ __forceinline__ void store16(void* p, const uint4 v) {
+  *reinterpret_cast<u32x4_any*>(p) = u32x4_any{v.x, v.y, v.z, v.w};
+}
+
+// the scales that go with 16 bytes of a row of A, from element d on
+template <typename A, typename S>
+__device__ __forceinline__ void scale_at(const S* __restrict__ scale, int d, float* f) {
+  if constexpr (sizeof(S) == 2 && sizeof(A) == 4) {
+    const u32x2_any v = *reinterpret_cast<const u32x2_any*>(scale + d);
+    f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NormRow<A>::kPiece; i += NormRow<S>::kPiece) NormRow<S>::unpack(load16(scale + d + i), f + i);
+  }
+}
+
+}  // namespace
+
 // The residual's addition and the norm of the sum: h = round_act(x + res), written to
 // hout, then rms_norm's arithmetic on h. Q8 = false: out = round_act((h * r) * scale), the
 // bits of k_rms_norm on h. Q8 = true: the same products in f32 to int8, with the row's
 // scale s = max(m / 127, FLT_MIN), m the largest magnitude (as an integer maximum of the f32
 // bits, which an infinity or a NaN tops: such a row gets s = NaN and zeros), and
-// q = rint(v * (1 / s)). One wave per row; hout may be x or res itself: a lane reads its
-// elements of both before it writes them. res NULL: h is x, and hout is not written.
-// pieces: rows move in 16-byte pieces (D a multiple of 64, every buffer aligned).
-template <typename A, typename S, bool Q8>
-__global__ __launch_bounds__(256) void k_add_rms_norm(int T, int D, float eps, int pieces, const A* x, const A* res,
-                                                       const S* __restrict__ scale, A* hout, A* __restrict__ out,
-                                                       int8_t* __restrict__ qout, float* __restrict__ qscale) {
+// q = rint(v * (1 / s)). hout may be x or res itself: a thread reads its elements of both
+// before it writes them. res NULL: h is x, and hout is not written.
+// Rows move in 16-byte pieces, of any alignment; the elements behind a row's last whole piece
+// one by one, by the row's first threads.
+// Bound by HBM for many rows, else by one row's round trip and its 64-step chain. W = 4 waves
+// share a row, W = 1 (narrow rows, many of them: add_rms_norm) leaves each to one wave:
+// bf16 16384 x 2048 47 us (5.7 TB/s) with four and 53 with one, one row 3.2 and 4.3; rows of
+// 512, 65536 of them, 84 with four and 48 with one (1000 of them 3.7 each).
+template <typename A, typename S, bool Q8, int W>
+__global__ __launch_bounds__(64 * kNormWaves) void k_add_rms_norm(int T, int D, float eps, const A* x, const A* res,
+                                                                   const S* __restrict__ scale, A* hout,
+                                                                   A* __restrict__ out, int8_t* __restrict__ qout,
+                                                                   float* __restrict__ qscale) {
 #pragma clang fp contract(off)
   using R = NormRow<A>;
+  constexpr int PT = W == 1 ? kNormNarrow / 64 : R::kPieces / W;  // pieces per thread of the widest row
+  constexpr int NT = 64 * W;          // threads of a row
+  constexpr int P = R::kPiece;
   extern __shared__ __attribute__((aligned(16))) uint8_t rows[];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int t = blockIdx.x * kNormWaves + w;
-  if (t >= T) return;  // per wave: this kernel has no block-wide barrier
-  A* row = reinterpret_cast<A*>(rows + (size_t)w * R::bytes(D));
-  const size_t at = (size_t)t * D;
-  const int n = D / R::kPiece;
-  uint4 v[R::kPieces];
-  if (pieces) {
-    uint4 o[R::kPieces];
+  __shared__ uint32_t factor[kNormWaves], largest[kNormWaves];  // W > 1: per row, per wave
+  const int wv = threadIdx.x >> 6, sub = wv / W, me = threadIdx.x - sub * NT;
+  const int t = blockIdx.x * (kNormWaves / W) + sub;
+  // rows past the last repeat it and store nothing (the waves of a block meet at barriers)
+  const bool live = t < T;
+  const size_t at = (size_t)(live ? t : T - 1) * D;
+  A* row = reinterpret_cast<A*>(rows + (size_t)sub * R::bytes(D));
+  const int n = D / P, end = n * P + me;  // this thread's element behind the pieces
+  const bool one = end < D;
+  uint4 v[PT], o[PT];
+  float sc[PT][P], h1 = 0.0f, s1 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < R::kPieces; ++i) {
-      v[i] = o[i] = uint4{0u, 0u, 0u, 0u};
-      if (lane + 64 * i < n) {
-        v[i] = reinterpret_cast<const uint4*>(x + at)[lane + 64 * i];
-        if (res) o[i] = reinterpret_cast<const uint4*>(res + at)[lane + 64 * i];
-      }
+  for (int i = 0; i < PT; ++i) {
+    const int p = me + NT * i;
+    if (p < n) {
+      v[i] = load16(x + at + p * P);
+      if (res) o[i] = load16(res + at + p * P);
+      scale_at<A, S>(scale, p * P, sc[i]);
     }
-#pragma unroll
-    for (int i = 0; i < R::kPieces; ++i) {
-      if (lane + 64 * i < n) {
-        if (res) {
-          float a[R::kPiece], b[R::kPiece];
-          R::unpack(v[i], a);
-          R::unpack(o[i], b);
-#pragma unroll
-          for (int j = 0; j < R::kPiece; ++j) a[j] = a[j] + b[j];
-          v[i] = R::pack(a);
-          reinterpret_cast<uint4*>(hout + at)[lane + 64 * i] = v[i];
-        }
-        *reinterpret_cast<uint4*>(row + R::at((lane + 64 * i) * R::kPiece)) = v[i];
-      }
-    }
-  } else {
-    for (int d = lane; d < D; d += 64) {
-      float h = Act<A>::load(x, at + d);
-      if (res) {
-        h = Act<A>::round(h + Act<A>::load(res, at + d));
-        Act<A>::store(hout, at + d, h);
-      }
-      Act<A>::store(row, R::at(d), h);
-    }
-    const int tail = (D - 1) / kRouterSlice * kRouterSlice + lane;
-    if (tail >= D) row[R::at(tail)] = 0;
   }
-  const float r = wave_rms_reduce(row, D, eps);
-  if constexpr (!Q8) {
-    if (pieces) {
+  if (one) {
+    h1 = Act<A>::load(x, at + end);
+    if (res) h1 = Act<A>::round(h1 + Act<A>::load(res, at + end));
+    s1 = Act<S>::load(scale, end);
+  }
 #pragma unroll
-      for (int i = 0; i < R::kPieces; ++i) {
-        const int p = lane + 64 * i;
-        if (p < n) {
-          float f[R::kPiece], sc[R::kPiece];
-          R::unpack(v[i], f);
-          scale_piece<A, S>(scale, p, sc);
+  for (int i = 0; i < PT; ++i) {
+    const int p = me + NT * i;
+    if (p < n) {
+      if (res) {
+        float a[P], b[P];
+        R::unpack(v[i], a);
+        R::unpack(o[i], b);
 #pragma unroll
-          for (int j = 0; j < R::kPiece; ++j) f[j] = rms_apply<A>(f[j], r, sc[j]);
-          reinterpret_cast<uint4*>(out + at)[p] = R::pack(f);
-        }
+        for (int j = 0; j < P; ++j) a[j] = a[j] + b[j];
+        v[i] = R::pack(a);
+        if (live) store16(hout + at + p * P, v[i]);
       }
-    } else {
-      for (int d = lane; d < D; d += 64)
-        Act<A>::store(out, at + d, rms_apply<A>(Act<A>::load(row, R::at(d)), r, Act<S>::load(scale, d)));
+      *reinterpret_cast<uint4*>(row + R::at(p * P)) = v[i];
     }
+  }
+  if (one) {
+    if (res && live) Act<A>::store(hout, at + end, h1);
+    Act<A>::store(row, R::at(end), h1);
+  }
+  // the last slice is filled up with zeros, whose squares leave its chain as it is
+  const int fill = (D - 1) / kRouterSlice * kRouterSlice + me;
+  if (me < kRouterSlice && fill >= D) row[R::at(fill)] = 0;
+  float r;
+  if constexpr (W == 1) {
+    r = wave_rms_reduce(row, D, eps);
+  } else {
+    __syncthreads();
+    if (me < 64) factor[sub] = __float_as_uint(wave_rms_reduce(row, D, eps));
+    __syncthreads();
+    r = __uint_as_float(factor[sub]);
+  }
+  if constexpr (!Q8) {
+    if (!live) return;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const int p = me + NT * i;
+      if (p < n) {
+        float f[P];
+        R::unpack(v[i], f);
+#pragma unroll
+        for (int j = 0; j < P; ++j) f[j] = rms_apply<A>(f[j], r, sc[i][j]);
+        store16(out + at + p * P, R::pack(f));
+      }
+    }
+    if (one) Act<A>::store(out, at + end, rms_apply<A>(h1, r, s1));
   } else {
     uint32_t m = 0;
-    auto value = [&](float h, float s) { return rms_apply<float>(h, r, s); };
-    auto note = [&](float f) { m = max(m, __float_as_uint(f) & 0x7fffffffu); };
-    if (pieces) {
+    float f[PT][P];
+    auto note = [&](float y) { m = max(m, __float_as_uint(y) & 0x7fffffffu); };
 #pragma unroll
-      for (int i = 0; i < R::kPieces; ++i) {
-        const int p = lane + 64 * i;
-        if (p < n) {
-          float f[R::kPiece], sc[R::kPiece];
-          R::unpack(v[i], f);
-          scale_piece<A, S>(scale, p, sc);
+    for (int i = 0; i < PT; ++i) {
+      if (me + NT * i < n) {
+        R::unpack(v[i], f[i]);
 #pragma unroll
-          for (int j = 0; j < R::kPiece; ++j) note(value(f[j], sc[j]));
-        }
+        for (int j = 0; j < P; ++j) note(f[i][j] = rms_apply<float>(f[i][j], r, sc[i][j]));
       }
-    } else {
-      for (int d = lane; d < D; d += 64) note(value(Act<A>::load(row, R::at(d)), Act<S>::load(scale, d)));
     }
+    const float f1 = rms_apply<float>(h1, r, s1);
+    if (one) note(f1);
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    for (int k = 32; k >= 1; k >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, k, 64));
+    if constexpr (W > 1) {
+      if ((threadIdx.x & 63) == 0) largest[wv] = m;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < W; ++k) m = max(m, largest[sub * W + k]);
+    }
+    if (!live) return;
     const bool bad = m > 0x7f7fffffu;
     const float s = fmaxf(__uint_as_float(m) / 127.0f, FLT_MIN);
     const float inv = bad ? 0.0f : 1.0f / s;
     // a bad row: (int)NaN would be the compiler's choice, so it is set apart
-    auto quant = [&](float f) {
-      const float y = fminf(fmaxf(rintf(f * inv), -127.0f), 127.0f);
-      return bad ? 0u : (uint32_t)(int)y & 0xffu;
+    auto quant = [&](float y) {
+      const float z = fminf(fmaxf(rintf(y * inv), -127.0f), 127.0f);
+      return bad ? 0u : (uint32_t)(int)z & 0xffu;
     };
-    if (pieces) {
 #pragma unroll
-      for (int i = 0; i < R::kPieces; ++i) {
-        const int p = lane + 64 * i;
-        if (p < n) {
-          float f[R::kPiece], sc[R::kPiece];
-          R::unpack(v[i], f);
-          scale_piece<A, S>(scale, p, sc);
-          uint32_t q[R::kPiece / 4];
+    for (int i = 0; i < PT; ++i) {
+      const int p = me + NT * i;
+      if (p < n) {
+        uint32_t q[P / 4];
 #pragma unroll
-          for (int j = 0; j < R::kPiece / 4; ++j) {
-            q[j] = 0;
+        for (int j = 0; j < P / 4; ++j) {
+          q[j] = 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) q[j] |= quant(value(f[4 * j + k], sc[4 * j + k])) << (8 * k);
-          }
-          if constexpr (R::kPiece == 8)
-            reinterpret_cast<uint2*>(qout + at)[p] = uint2{q[0], q[1]};
-          else
-            reinterpret_cast<uint32_t*>(qout + at)[p] = q[0];
+          for (int k = 0; k < 4; ++k) q[j] |= quant(f[i][4 * j + k]) << (8 * k);
         }
+        if constexpr (P == 8)
+          *reinterpret_cast<u32x2_any*>(qout + at + p * P) = u32x2_any{q[0], q[1]};
+        else
+          *reinterpret_cast<u32_any*>(qout + at + p * P) = q[0];
       }
-    } else {
-      for (int d = lane; d < D; d += 64)
-        qout[at + d] = (int8_t)quant(value(Act<A>::load(row, R::at(d)), Act<S>::load(scale, d)));
     }
-    if (lane == 0) qscale[t] = bad ? __builtin_nanf("") : s;
+    if (one) qout[at + end] = (int8_t)quant(f1);
+    if (me == 0) qscale[t] = bad ? __builtin_nanf("") : s;
   }
 }
 
@@ -238,23 +282,31 @@ using namespace kmoe;
 
 namespace {
 
+template <typename A, typename S, int W>
+void add_rms_norm_of(const kmoe_desc& d, const void* x, const void* res, const void* scale, float eps, void* hout,
+                     void* out, int8_t* q, float* qscale, hipStream_t st) {
+  const int T = (int)d.tokens, D = (int)d.hidden, per = kNormWaves / W;
+  const dim3 grid((T + per - 1) / per), block(64 * kNormWaves);
+  const size_t lds = per * NormRow<A>::bytes(D);
+  if (q)
+    hipLaunchKernelGGL((k_add_rms_norm<A, S, true, W>), grid, block, lds, st, T, D, eps, reinterpret_cast<const A*>(x),
+                       reinterpret_cast<const A*>(res), reinterpret_cast<const S*>(scale), reinterpret_cast<A*>(hout),
+                       reinterpret_cast<A*>(out), q, qscale);
+  else
+    hipLaunchKernelGGL((k_add_rms_norm<A, S, false, W>), grid, block, lds, st, T, D, eps, reinterpret_cast<const A*>(x),
+                       reinterpret_cast<const A*>(res), reinterpret_cast<const S*>(scale), reinterpret_cast<A*>(hout),
+                       reinterpret_cast<A*>(out), q, qscale);
+}
+
 template <typename A, typename S>
 void add_rms_norm(const kmoe_desc& d, const void* x, const void* res, const void* scale, float eps, void* hout,
                   void* out, int8_t* q, float* qscale, hipStream_t st) {
-  const int T = (int)d.tokens, D = (int)d.hidden;
-  const bool pieces = D % kRouterSlice == 0 && aligned16(x) && aligned16(res) && aligned16(scale) && aligned16(hout) &&
-                      aligned16(out) && aligned16(q);
-  const dim3 grid((T + kNormWaves - 1) / kNormWaves), block(64 * kNormWaves);
-  const size_t lds = kNormWaves * NormRow<A>::bytes(D);
-  if (q)
-    hipLaunchKernelGGL((k_add_rms_norm<A, S, true>), grid, block, lds, st, T, D, eps, (int)pieces,
-                       reinterpret_cast<const A*>(x), reinterpret_cast<const A*>(res),
-                       reinterpret_cast<const S*>(scale), reinterpret_cast<A*>(hout), (A*)nullptr, q, qscale);
+  // four waves per row spread a row's latency (64 rows of 4096: 3.9 us, one wave each 6.2),
+  // but of narrow rows they leave most threads idle (see the kernel's figures)
+  if (d.tokens > kNormManyRows && d.hidden <= kNormNarrow * NormRow<A>::kPiece)
+    add_rms_norm_of<A, S, 1>(d, x, res, scale, eps, hout, out, q, qscale, st);
   else
-    hipLaunchKernelGGL((k_add_rms_norm<A, S, false>), grid, block, lds, st, T, D, eps, (int)pieces,
-                       reinterpret_cast<const A*>(x), reinterpret_cast<const A*>(res),
-                       reinterpret_cast<const S*>(scale), reinterpret_cast<A*>(hout), reinterpret_cast<A*>(out),
-                       (int8_t*)nullptr, (float*)nullptr);
+    add_rms_norm_of<A, S, kNormWaves>(d, x, res, scale, eps, hout, out, q, qscale, st);
 }
 
 }  // namespace

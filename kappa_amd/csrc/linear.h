@@ -16,7 +16,8 @@ constexpr int kLoraRankPad = 32;       // ranks of one step of the expanding pro
 constexpr int kLoraMaxRank = 256;
 constexpr int kLoraMaxAdapters = 1024;
 constexpr int kLoraSortBlock = 512;    // tokens per block of the sort
-constexpr int kLinearDecodeTokens = 64;  // the streaming kernel's largest batch
+constexpr int kLinearDecodeTokens = 64;  // above: the GEMM
+constexpr int kSplitSteps = 8;         // 128-byte steps of the rows that a block of the two-launch form takes
 
 }  // namespace kmoe
 
@@ -33,11 +34,19 @@ inline int64_t step_of(kmoe_dtype x) { return enum_value(x) == KMOE_DTYPE_I8 ? 1
 // Other rows are copied into the workspace first, padded with zeros.
 bool linear_rows_fit(const kmoe_linear_weight& w, const void* x, kmoe_dtype x_dtype, int64_t x_stride);
 
-// Byte offsets of the workspace: the copied rows (0), the adapters' inner values.
+// Whether a call of up to 64 tokens without adapters takes the two-launch form: the rows'
+// padded bytes exceed what every block of the single launch reads well (linear.hip).
+bool linear_splits(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype);
+
+// Byte offsets of the workspace: the copied rows (0, where they are copied), partial sums
+// (two-launch form), the adapters' inner values.
 struct LinearSpace {
-  size_t u, total;
+  size_t part, u, total;
 };
-LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora);
+LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora,
+                         bool copied);
+// The largest of any call of up to `tokens` rows
+size_t linear_most_bytes(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora);
 
 kmoe_status check_linear_weight(const kmoe_linear_weight* w, bool buffers);
 kmoe_status check_lora(const kmoe_lora* lora, bool buffers);
@@ -52,6 +61,8 @@ kmoe_status validate_lora_sort(const int32_t* adapter, const kmoe_lora_batch* ba
                                size_t scratch_bytes);
 kmoe_status validate_linear_workspace_bytes(const kmoe_linear_weight* w, int64_t tokens, kmoe_dtype x_dtype,
                                             const kmoe_lora* lora, size_t* bytes);
+kmoe_status validate_linear_call_bytes(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                                       int64_t x_stride, const kmoe_lora* lora, size_t* bytes);
 kmoe_status validate_linear(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
                             int64_t x_stride, const float* x_scale, const kmoe_lora* lora,
                             const kmoe_lora_batch* batch, const void* out, const void* workspace,

@@ -9,6 +9,8 @@
 // Three kinds of products (Kind): bf16 rows with bf16 or int8 weights on
 // v_mfma_f32_16x16x32_bf16 (int8 becomes bf16 in registers, exactly), and int8 rows
 // with int8 weights on v_mfma_i32_16x16x64_i8, whose sums are exact.
+#include <type_traits>
+
 #include "common.h"
 #include "expert_dev.h"
 #include "linear_launch.h"
@@ -40,6 +42,7 @@ struct LinearArgs {
   const char* b;      // [L][out/16][rank/32][4][16][8]
   const float* factor;
   int rank, rp, kcp;  // rank, rank padded, 64-deep chunks of the packed A
+  floatx4* part;      // up to 64 tokens: [splits][T][out/4] partial sums
   void* u;            // up to 64 tokens f32 [T][rp]; above, bf16 [T][rp/32][hi 32 | lo 32] in sorted order
 };
 
@@ -250,24 +253,23 @@ __global__ __launch_bounds__(kLoraSortBlock) void k_lora_sort(int T, int L, cons
 }
 
 // ---------------------------------------------------------------------------
-// u = factor x A for few tokens: one block per token and 16 ranks, 16 waves over the chunks.
+// u = factor x A for few tokens, a block's share: 16 ranks (group g) of token t, NW waves
+// over the chunks.
 // ---------------------------------------------------------------------------
-template <int KIND>
-__global__ __launch_bounds__(1024) void k_lora_shrink_rows(LinearArgs p) {
-  __shared__ float red[16][16];
+template <int KIND, int NW>
+__device__ __forceinline__ void shrink_row(const LinearArgs& p, int t, int g, float (*red)[16]) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q = lane >> 4;
-  const int t = blockIdx.x, g = blockIdx.y;
   const int ad = p.adapter[t];
   if (ad < 0) return;  // the whole block
+  const float f = p.factor[ad] * (KIND == kII ? p.xs[t] : 1.0f);
   const char* xr = p.x + (size_t)t * p.row_bytes + q * (KIND == kII ? 16 : 32);
   const char* ar = p.a + (size_t)ad * p.rp * p.kcp * 128 + (size_t)g * p.kcp * 2048 + lane * 16;
   float acc = 0.0f;
-  for (int kc = wv; kc < p.kc; kc += 16) {
-    const uint4 a0 = *reinterpret_cast<const uint4*>(ar + (size_t)kc * 2048);
-    const uint4 a1 = *reinterpret_cast<const uint4*>(ar + (size_t)kc * 2048 + 1024);
+#pragma unroll 4
+  for (int kc = wv; kc < p.kc; kc += NW) {
     float fa[16], fx[16];
-    unpack8(a0, fa);
-    unpack8(a1, fa + 8);
+    unpack8(*reinterpret_cast<const uint4*>(ar + (size_t)kc * 2048), fa);
+    unpack8(*reinterpret_cast<const uint4*>(ar + (size_t)kc * 2048 + 1024), fa + 8);
     if constexpr (KIND == kII) {
       const uint4 v = *reinterpret_cast<const uint4*>(xr + kc * 64);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -286,87 +288,124 @@ __global__ __launch_bounds__(1024) void k_lora_shrink_rows(LinearArgs p) {
   __syncthreads();
   if (threadIdx.x < 16) {
     float s = 0.0f;
-    for (int w = 0; w < 16; ++w) s += red[w][threadIdx.x];
-    s *= p.factor[ad];
-    if (KIND == kII) s *= p.xs[t];
-    reinterpret_cast<float*>(p.u)[(size_t)t * p.rp + g * 16 + threadIdx.x] = s;
+    for (int w = 0; w < NW; ++w) s += red[w][threadIdx.x];
+    reinterpret_cast<float*>(p.u)[(size_t)t * p.rp + g * 16 + threadIdx.x] = s * f;
   }
 }
 
 // ---------------------------------------------------------------------------
-// u for many tokens, 16 sorted rows per block: MFMA, eight waves over the chunks, one
-// pass per adapter of the tile; u as bf16 hi + lo.
+// u for many tokens, 16 sorted rows per block: MFMA, sixteen waves over the chunks, one
+// pass per adapter of the tile and NG groups of 16 ranks; u as bf16 hi + lo. Bound by
+// latency: the tile's adapters come with its rows, and all chunks of 4096 elements are in
+// flight together.
 // ---------------------------------------------------------------------------
-template <int KIND>
-__global__ __launch_bounds__(512) void k_lora_shrink(LinearArgs p) {
-  constexpr int NG = 4;  // groups of 16 ranks at a time
-  __shared__ floatx4 red[8][NG][64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
-  const int r0 = blockIdx.x * 16, r1 = min(r0 + 16, p.T);
-  const int row = p.order[min(r0 + c, p.T - 1)];
-  const char* xr = p.x + (size_t)row * p.row_bytes + q * (KIND == kII ? 16 : 32);
+template <int KIND, int NG>
+__global__ __launch_bounds__(1024) void k_lora_shrink(LinearArgs p) {
+  constexpr int NW = 16;
+  constexpr int CB = NG == 1 ? 4 : 2;  // chunks whose loads are in flight together (128 registers)
+  constexpr int XL = KIND == kII ? 1 : 2;
+  __shared__ floatx4 red[NW][NG][64];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
+  const int r0 = blockIdx.x * 16, at = min(r0 + c, p.T - 1);
+  const int row = p.order[at];
+  const int mine = r0 + c < p.T ? p.sorted[at] : -1;
+  const char* const xr = p.x + (size_t)row * p.row_bytes + q * (16 * XL);
   const float xs = KIND == kII ? p.xs[row] : 1.0f;
-  const int groups = p.rp >> 4;
-  for (int pos = r0; pos < r1;) {
-    const int ad = p.sorted[pos];
-    if (ad < 0) break;
-    const int end = min(max(p.offsets[ad + 1], pos + 1), r1);
-    const float f = p.factor[ad];
+  const int groups = (p.rank + 15) >> 4;
+  uint4 x[CB][XL];
+  auto load_x = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+      if (kb + NW * i < p.kc) {
+#pragma unroll
+        for (int l = 0; l < XL; ++l) x[i][l] = *reinterpret_cast<const uint4*>(xr + (kb + NW * i) * (64 * XL) + l * 16);
+      }
+    }
+  };
+  // up to NW * CB chunks the rows stay in registers for every adapter and group
+  const bool once = p.kc <= NW * CB;
+  load_x(wv);
+  uint64_t left = __ballot(mine >= 0);  // the tile's rows whose adapter is still to come
+  while (left) {
+    const int ad = __shfl(mine, __ffsll((unsigned long long)left) - 1, 64);
+    const uint64_t these = __ballot(mine == ad);
+    left &= ~these;
+    const float f = p.factor[ad] * xs;
+    uint16_t* const u = reinterpret_cast<uint16_t*>(p.u) + (size_t)(r0 + c) * p.rp * 2;
+    // ranks r .. r + 3 of this lane's row
+    auto put = [&](int r, const floatx4 v) {
+      uint16_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split_bf16(v[j], hi[j], lo[j]);
+      uint16_t* d = u + (r >> 5) * 64 + (r & 31);
+      *reinterpret_cast<uint2*>(d) = uint2{hi[0] | (uint32_t)hi[1] << 16, hi[2] | (uint32_t)hi[3] << 16};
+      *reinterpret_cast<uint2*>(d + 32) = uint2{lo[0] | (uint32_t)lo[1] << 16, lo[2] | (uint32_t)lo[3] << 16};
+    };
     for (int g0 = 0; g0 < groups; g0 += NG) {
       const char* ar = p.a + (size_t)ad * p.rp * p.kcp * 128 + (size_t)g0 * p.kcp * 2048 + lane * 16;
       floatx4 acc[NG];
 #pragma unroll
       for (int g = 0; g < NG; ++g) acc[g] = floatx4{0.f, 0.f, 0.f, 0.f};
-      for (int kc = wv; kc < p.kc; kc += 8) {
-        bf16x8 x0, x1;
-        if constexpr (KIND == kII) {
-          cvt16(*reinterpret_cast<const uint4*>(xr + kc * 64), x0, x1);
-        } else {
-          x0 = as_bf16x8(*reinterpret_cast<const uint4*>(xr + kc * 128));
-          x1 = as_bf16x8(*reinterpret_cast<const uint4*>(xr + kc * 128 + 16));
+      for (int kb = wv; kb < p.kc; kb += NW * CB) {
+        uint4 a[CB][NG][2];
+        if (!once) load_x(kb);
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+          const int kc = kb + NW * i;
+          if (kc < p.kc) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              // (a group past the last reads the last again; its sum is not used)
+              const char* src = ar + ((size_t)min(g, groups - 1 - g0) * p.kcp + kc) * 2048;
+              a[i][g][0] = *reinterpret_cast<const uint4*>(src);
+              a[i][g][1] = *reinterpret_cast<const uint4*>(src + 1024);
+            }
+          }
         }
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          if (g0 + g < groups) {
-            const char* at = ar + ((size_t)g * p.kcp + kc) * 2048;
-            acc[g] = mfma16(as_bf16x8(*reinterpret_cast<const uint4*>(at)), x0, acc[g]);
-            acc[g] = mfma16(as_bf16x8(*reinterpret_cast<const uint4*>(at + 1024)), x1, acc[g]);
+        for (int i = 0; i < CB; ++i) {
+          if (kb + NW * i < p.kc) {
+            bf16x8 x0, x1;
+            if constexpr (KIND == kII) {
+              cvt16(x[i][0], x0, x1);
+            } else {
+              x0 = as_bf16x8(x[i][0]);
+              x1 = as_bf16x8(x[i][XL - 1]);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+              acc[g] = mfma16(as_bf16x8(a[i][g][1]), x1, mfma16(as_bf16x8(a[i][g][0]), x0, acc[g]));
           }
         }
       }
 #pragma unroll
       for (int g = 0; g < NG; ++g) red[wv][g][lane] = acc[g];
       __syncthreads();
-      if (wv < NG && g0 + wv < groups && r0 + c >= pos && r0 + c < end) {
+      if (wv < NG && g0 + wv < groups && mine == ad) {
         floatx4 s = red[0][wv][lane];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) s += red[w][wv][lane];
-        // ranks 4 q .. 4 q + 3 of group g0 + wv
-        const int r = (g0 + wv) * 16 + 4 * q;
-        uint16_t* u = reinterpret_cast<uint16_t*>(p.u) + (size_t)(r0 + c) * p.rp * 2 + (r >> 5) * 64 + (r & 31);
-        uint16_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split_bf16(s[j] * xs * f, hi[j], lo[j]);
-        *reinterpret_cast<uint2*>(u) = uint2{hi[0] | (uint32_t)hi[1] << 16, hi[2] | (uint32_t)hi[3] << 16};
-        *reinterpret_cast<uint2*>(u + 32) = uint2{lo[0] | (uint32_t)lo[1] << 16, lo[2] | (uint32_t)lo[3] << 16};
+        for (int w = 1; w < NW; ++w) s += red[w][wv][lane];
+        put((g0 + wv) * 16 + 4 * q, s * f);
       }
       __syncthreads();
     }
-    pos = end;
+    // the padding's ranks meet zeros of B, so they have to be finite
+    if ((groups & 1) && wv == NW - 1 && mine == ad) put(groups * 16 + 4 * q, floatx4{0.f, 0.f, 0.f, 0.f});
   }
 }
 
 // ---------------------------------------------------------------------------
-// Up to 64 tokens: the weights stream through registers once. A block takes 16 CG
-// columns for all rows, its eight waves the chunks in turn parts; the partial sums meet
-// in LDS in wave order. Each thread then finishes four columns of a row, with the
-// adapters' part in f32.
+// Few tokens without adapters: the weights stream through registers once. A block takes 16 CG
+// columns for all rows, its eight waves an eighth of the chunks each; the partial sums meet
+// in LDS in wave order. Bound by latency: a wave requests NB chunks at once (the whole of its
+// share up to 2048 inputs).
 // ---------------------------------------------------------------------------
 template <int KIND, int RB, int CG>
 __global__ __launch_bounds__(512) void k_linear_decode(LinearArgs p) {
-  constexpr int NB = 2;
   constexpr int WL = KIND == kBB ? 2 : 1;   // 16-byte weight loads per chunk and group
   constexpr int XL = KIND == kII ? 1 : 2;   // and row loads per chunk and row block
+  constexpr int kFit = 40 / (CG * WL + RB * XL);  // chunks in flight: at most 160 registers
+  constexpr int NB = kFit > 4 ? 4 : kFit;
   __shared__ floatx4 red[8][CG][RB][64];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, q = lane >> 4;
@@ -446,64 +485,207 @@ __global__ __launch_bounds__(512) void k_linear_decode(LinearArgs p) {
   float v[4];
   const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + col);
   if constexpr (KIND == kII) {
-    int32x4 s = {0, 0, 0, 0};
+    int32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += __builtin_bit_cast(int32x4, red[w][g][b][lane]);
+    for (int k = 0; k < 8; ++k) sum += __builtin_bit_cast(int32x4, red[k][g][b][lane]);
     const float xs = p.xs[row];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (float)s[j] * xs * sc[j];
+    for (int j = 0; j < 4; ++j) v[j] = (float)sum[j] * xs * sc[j];
   } else {
-    floatx4 s = red[0][g][b][lane];
+    floatx4 sum = red[0][g][b][lane];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) s += red[w][g][b][lane];
+    for (int k = 1; k < 8; ++k) sum += red[k][g][b][lane];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = s[j] * sc[j];
-  }
-  if (p.adapter) {
-    const int ad = p.adapter[row];
-    if (ad >= 0) {
-      const float* u = reinterpret_cast<const float*>(p.u) + (size_t)row * p.rp;
-      const char* bb = p.b + ((size_t)ad * p.cgs + cg) * (p.rp * 32) + q * 64;
-      for (int r = 0; r < p.rank; r += 8) {
-        const floatx4 u0 = *reinterpret_cast<const floatx4*>(u + r), u1 = *reinterpret_cast<const floatx4*>(u + r + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float f[8];
-          unpack8(*reinterpret_cast<const uint4*>(bb + r * 32 + j * 16), f);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[j] = __builtin_fmaf(u0[k], f[k], v[j]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[j] = __builtin_fmaf(u1[k], f[4 + k], v[j]);
-        }
-      }
-    }
+    for (int j = 0; j < 4; ++j) v[j] = sum[j] * sc[j];
   }
   store4(p.out + (size_t)row * p.N, col, p.N, (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0, v);
 }
 
 // ---------------------------------------------------------------------------
+// Few tokens in two launches. The first: blocks of 128 columns and eight steps (128 bytes of
+// each row), every load of a block in flight at once - the rows through LDS, shared by NW
+// waves of 16 CG columns, the weights in registers - whose partial sums go to the workspace;
+// and beside them the blocks of the adapters' u, which thus costs no launch of its own. The
+// second adds the partial sums in order and the adapters' part, and rounds.
+// 64 rows with 32 adapters of rank 16, 2048 -> 5120: 14.2 us, of which the second 4; the
+// weights, adapters and rows alone would take 4 us of HBM. With u in a launch of its own and the
+// adapters' part in the single launch above it took 19.7.
+// ---------------------------------------------------------------------------
+template <int KIND, int RB, int NW, int CG>
+__global__ __launch_bounds__(64 * NW) void k_linear_split(LinearArgs p, int splits, int shrink_blocks) {
+  constexpr int ST = kSplitSteps;
+  constexpr int WL = KIND == kBI ? 1 : 2;        // 16-byte weight loads per step and group
+  constexpr int SA = RB * 16 * 128;              // a step's rows
+  constexpr int AJ = RB * 2;                     // loads of a step: 8 rows each
+  constexpr int kOrder = KIND == kII ? 0 : 1;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[ST * SA];
+  // u first: its blocks take longest
+  if ((int)blockIdx.x < shrink_blocks) {
+    const int groups = (p.rank + 15) >> 4;
+    shrink_row<KIND, NW>(p, blockIdx.x / groups, blockIdx.x % groups, reinterpret_cast<float(*)[16]>(smem));
+    return;
+  }
+  const int block = blockIdx.x - shrink_blocks;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, q = lane >> 4;
+  const int split = block % splits, cg0 = (block / splits) * (NW * CG) + wv * CG;
+  const int steps = KIND == kII ? (p.kc + 1) >> 1 : p.kc;
+  const int s0 = split * ST, n = min(ST, steps - s0);
+  const uint32_t lds0 = lds_addr(smem);
+  uint4 w[ST][CG][WL];
+#pragma unroll
+  for (int i = 0; i < ST; ++i) {
+    if (i < n) {
+#pragma unroll
+      for (int g = 0; g < CG; ++g)
+#pragma unroll
+        for (int l = 0; l < WL; ++l)
+          w[i][g][l] = load_stream16(reinterpret_cast<const int8_t*>(p.w) +
+                                     (size_t)min(cg0 + g, p.cgs - 1) * p.cg_bytes + (size_t)(s0 + i) * (1024 * WL) +
+                                     l * 1024 + lane * 16);
+    }
+  }
+  // the loads of all steps' rows, shared out over the waves
+#pragma unroll
+  for (int j = 0; j < (ST * AJ + NW - 1) / NW; ++j) {
+    const int i = (wv + NW * j) / AJ, r8 = (wv + NW * j) % AJ;
+    if (i < n) {
+      const int r = 8 * r8 + (lane >> 3);
+      const uint32_t off = (uint32_t)min(r, p.T - 1) * p.row_bytes + (uint32_t)(a_piece_at<kOrder>(r, lane & 7) * 16);
+      dma16(off, p.x + (size_t)(s0 + i) * 128, __builtin_amdgcn_readfirstlane(lds0 + i * SA + r8 * 1024));
+    }
+  }
+  floatx4 acc[CG][RB];
+  int32x4 iacc[CG][RB];
+#pragma unroll
+  for (int g = 0; g < CG; ++g)
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      acc[g][b] = floatx4{0.f, 0.f, 0.f, 0.f};
+      iacc[g][b] = int32x4{0, 0, 0, 0};
+    }
+  vm_barrier<0>();
+#pragma unroll
+  for (int i = 0; i < ST; ++i) {
+    if (i < n) {
+      const uint16_t* As = reinterpret_cast<const uint16_t*>(smem + i * SA);
+      bf16x8 f[CG][2];
+#pragma unroll
+      for (int g = 0; g < CG; ++g) {
+        if constexpr (KIND == kBI) {
+          cvt16(w[i][g][0], f[g][0], f[g][1]);
+        } else {
+          f[g][0] = as_bf16x8(w[i][g][0]);
+          f[g][1] = as_bf16x8(w[i][g][WL - 1]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const bf16x8 a =
+              *reinterpret_cast<const bf16x8*>(As + a_at<kOrder>(b * 16 + c, KIND == kII ? 4 * st + q : 2 * q + st));
+#pragma unroll
+          for (int g = 0; g < CG; ++g) {
+            if constexpr (KIND == kII)
+              iacc[g][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int32x4, f[g][st]),
+                                                                 __builtin_bit_cast(int32x4, a), iacc[g][b], 0, 0, 0);
+            else
+              acc[g][b] = mfma16(f[g][st], a, acc[g][b]);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < CG; ++g) {
+    if (cg0 + g >= p.cgs) continue;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const int row = b * 16 + c;
+      if (row < p.T)
+        p.part[((size_t)split * p.T + row) * (p.cgs * 4) + (cg0 + g) * 4 + q] =
+            KIND == kII ? __builtin_bit_cast(floatx4, iacc[g][b]) : acc[g][b];
+    }
+  }
+}
+
+// One wave: 256 columns of a row, four per lane, so that the adapter's B is read in whole
+// lines (a wave on 16 columns of 16 rows, which its sums would come to more easily, took
+// 23 us instead of 19.6 for 24 rows of rank 64, 4096 -> 9216).
+template <int KIND>
+__global__ __launch_bounds__(64) void k_linear_finish(LinearArgs p, int splits) {
+  const int quad = blockIdx.x * 64 + threadIdx.x, row = blockIdx.y, cg = quad >> 2, q = quad & 3;
+  if (cg >= p.cgs) return;
+  const int ad = p.adapter ? p.adapter[row] : -1;
+  const floatx4* part = p.part + (size_t)row * (p.cgs * 4) + quad;
+  const size_t pitch = (size_t)p.T * (p.cgs * 4);
+  const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + quad * 4);
+  float v[4];
+  if constexpr (KIND == kII) {
+    int32x4 sum = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) sum += __builtin_bit_cast(int32x4, part[k * pitch]);
+    const float xs = p.xs[row];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (float)sum[j] * xs * sc[j];
+  } else {
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) sum += part[k * pitch];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = sum[j] * sc[j];
+  }
+  if (ad >= 0) {
+    const float* const u = reinterpret_cast<const float*>(p.u) + (size_t)row * p.rp;
+    const char* const bb = p.b + ((size_t)ad * p.cgs + cg) * (p.rp * 32) + q * 64;
+    floatx4 extra = {0.f, 0.f, 0.f, 0.f};
+    const int r8 = (p.rank + 7) >> 3;
+#pragma unroll 4
+    for (int s = 0; s < r8; ++s) {
+      const floatx4 u0 = *reinterpret_cast<const floatx4*>(u + s * 8), u1 = *reinterpret_cast<const floatx4*>(u + s * 8 + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[8];
+        unpack8(*reinterpret_cast<const uint4*>(bb + s * 256 + j * 16), f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) extra[j] = __builtin_fmaf(u0[k], f[k], extra[j]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) extra[j] = __builtin_fmaf(u1[k], f[4 + k], extra[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += extra[j];
+  }
+  store4(p.out + (size_t)row * p.N, quad * 4, p.N, (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0, v);
+}
+
+// ---------------------------------------------------------------------------
 // Above 64 tokens: a GEMM over tiles of BM rows and BN columns. Steps of 128 bytes of
 // every row (64 bf16, 128 int8) and the columns' weights of the same depth reach LDS by direct
-// loads, two stages. Rows as [row][8 x 16 B] with the pieces swizzled by row
+// loads, a ring of NS stages. Rows as [row][8 x 16 B] with the pieces swizzled by row
 // (a_piece_at), the weights in the packed order, which is the order their lanes read. The
 // weights are the MFMA's first operand: a lane ends with four consecutive columns.
+// A step is two halves, and each half's fragments are read while the MFMAs of the half before
+// run (the order is held by scheduling groups); the one barrier of a step stands between
+// them, where the stage has been read and the next one has landed.
 //
 // With adapters the rows are the sorted ones, so a tile meets few adapters. After the
-// base sum, already scaled to f32, each adapter of the tile adds steps of 32 ranks: the
-// tile's rows of u (hi and lo, 128 bytes) times the adapter's B. A 16-row group that lies
-// wholly in the adapter's range adds in place; one that does not computes the product
-// apart and takes its own rows by selection, so that nothing of another adapter (an infinity
-// times zero) reaches a row.
+// base sum, scaled to f32, each adapter of the tile adds steps of 32 ranks in the same
+// ring: the tile's rows of u (hi and lo, 128 bytes) times the adapter's B. A 16-row group
+// that lies wholly in the adapter's range adds in place; one that does not computes the
+// product apart and takes its own rows by selection, so that nothing of another adapter (an
+// infinity times zero) reaches a row.
 // ---------------------------------------------------------------------------
-template <int KIND, int WM, int WN, int MI, int NI, bool LORA>
-__global__ __launch_bounds__(64 * WM * WN) void k_linear_gemm(LinearArgs p, int tm, int tn) {
+template <int KIND, int WM, int WN, int MI, int NI, int NS, bool LORA>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_linear_gemm(LinearArgs p, int tm, int tn) {
   constexpr int NW = WM * WN, BM = 16 * WM * MI, BN = 16 * WN * NI;
   constexpr int BB = KIND == kBI ? 1024 : 2048;  // weight bytes of a column group per step
-  constexpr int SA = BM * 128, SB = BN / 16 * BB;
-  constexpr int AJ = BM / 8 / NW, BJ = SB / 1024 / NW;
+  constexpr int SA = BM * 128, SB = BN / 16 * BB, SS = SA + SB;
+  constexpr int AJ = BM / 8 / NW, BJ = SB / 1024 / NW, PER = AJ + BJ;
   static_assert(BM % (8 * NW) == 0 && SB % (1024 * NW) == 0 && BN / 16 % NW == 0, "whole loads per wave");
   constexpr int kOrder = KIND == kII ? 0 : 1;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * (SA + SB)];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NS * SS];
+  __shared__ int seg[LORA ? 3 : 1][LORA ? BM : 1];  // per tile row: token, adapter, where the adapter's rows end
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, q = lane >> 4;
   const int wm = wv / WN, wn = wv % WN;
@@ -516,14 +698,16 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_gemm(LinearArgs p, int 
   const int r0 = mt * BM, rows = min(BM, p.T - r0);
   const int cg0 = nt * (BN / 16);
   const uint32_t lds0 = lds_addr(smem);
+  auto stage_at = [&](int s, int off) { return __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)((s % NS) * SS + off)); };
 
-  uint32_t aoff[AJ];
-#pragma unroll
-  for (int j = 0; j < AJ; ++j) {
-    const int r = 8 * (wv + NW * j) + (lane >> 3);
-    const int pos = min(r0 + r, p.T - 1);
-    const int row = LORA ? p.order[pos] : pos;
-    aoff[j] = (uint32_t)row * p.row_bytes + (uint32_t)(a_piece_at<kOrder>(r, lane & 7) * 16);
+  if constexpr (LORA) {
+    for (int r = tid; r < BM; r += 64 * NW) {
+      const int pos = min(r0 + r, p.T - 1);
+      const int ad = r < rows ? p.sorted[pos] : -1;
+      seg[0][r] = p.order[pos];
+      seg[1][r] = ad;
+      seg[2][r] = ad < 0 ? rows : min(max(p.offsets[ad + 1] - r0, r + 1), rows);
+    }
   }
   const char* bsrc[BJ];
 #pragma unroll
@@ -531,146 +715,233 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_gemm(LinearArgs p, int 
     const int at = (wv + NW * j) * 1024;
     bsrc[j] = p.w + (size_t)min(cg0 + at / BB, p.cgs - 1) * p.cg_bytes + at % BB;
   }
+  if constexpr (LORA) __syncthreads();
+  uint32_t aoff[AJ];
+#pragma unroll
+  for (int j = 0; j < AJ; ++j) {
+    const int r = 8 * (wv + NW * j) + (lane >> 3);
+    int row = min(r0 + r, p.T - 1);
+    if constexpr (LORA) row = seg[0][r];
+    aoff[j] = (uint32_t)row * p.row_bytes + (uint32_t)(a_piece_at<kOrder>(r, lane & 7) * 16);
+  }
   auto issue = [&](int s) {
-    const uint32_t st = lds0 + (uint32_t)((s & 1) * (SA + SB));
 #pragma unroll
-    for (int j = 0; j < AJ; ++j) dma16(aoff[j], p.x + (size_t)s * 128, st + (wv + NW * j) * 1024);
+    for (int j = 0; j < BJ; ++j)
+      dma16(lane * 16, bsrc[j] + (size_t)s * BB, stage_at(s, SA + (wv + NW * j) * 1024));
 #pragma unroll
-    for (int j = 0; j < BJ; ++j) dma16(lane * 16, bsrc[j] + (size_t)s * BB, st + SA + (wv + NW * j) * 1024);
+    for (int j = 0; j < AJ; ++j) dma16(aoff[j], p.x + (size_t)s * 128, stage_at(s, (wv + NW * j) * 1024));
   };
+  // the adapters' steps: `at` is the tile row where the adapter starts (rows: none left)
+  struct Cursor {
+    int at, ad, end, s;
+  };
+  const int rb = LORA ? p.rp >> 5 : 0;
+  auto enter = [&](Cursor& k, int at) {
+    k.at = at;
+    k.s = 0;
+    if (at < rows) {
+      k.ad = __builtin_amdgcn_readfirstlane(seg[LORA ? 1 : 0][LORA ? at : 0]);
+      k.end = __builtin_amdgcn_readfirstlane(seg[LORA ? 2 : 0][LORA ? at : 0]);
+      if (k.ad < 0) k.at = rows;
+    }
+  };
+  auto advance = [&](Cursor& k) {
+    if (++k.s == rb) enter(k, k.end);
+  };
+  const char* const ubase = reinterpret_cast<const char*>(p.u) + (size_t)r0 * rb * 128;
+  auto issue_lora = [&](const Cursor& k, int s) {
+    constexpr int LB = BN / 16 / NW;
+#pragma unroll
+    for (int j = 0; j < LB; ++j) {
+      const int cg = min(cg0 + wv + NW * j, p.cgs - 1);
+      dma16(lane * 16, p.b + (((size_t)k.ad * p.cgs + cg) * rb + k.s) * 1024, stage_at(s, SA + (wv + NW * j) * 1024));
+    }
+#pragma unroll
+    for (int j = 0; j < AJ; ++j) {
+      const int r = 8 * (wv + NW * j) + (lane >> 3);
+      dma16((uint32_t)min(r, rows - 1) * (uint32_t)(rb * 128) + (uint32_t)(a_piece_at<1>(r, lane & 7) * 16),
+            ubase + k.s * 128, stage_at(s, (wv + NW * j) * 1024));
+    }
+  };
+  Cursor next{rows, -1, rows, 0}, cur{rows, -1, rows, 0};
+  int issued = 0;  // adapters' steps; the k-th takes the ring's stage as base step steps + k would
+  if constexpr (LORA) {
+    enter(next, 0);
+    cur = next;
+  }
+
   floatx4 acc[MI][NI];
-  const int steps = KIND == kII ? (p.kc + 1) >> 1 : p.kc;
-  {
-    int32x4 iacc[KIND == kII ? MI : 1][KIND == kII ? NI : 1];
+  int32x4 iacc[KIND == kII ? MI : 1][KIND == kII ? NI : 1];
+#pragma unroll
+  for (int m = 0; m < MI; ++m)
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (KIND == kII) iacc[m][n] = int32x4{0, 0, 0, 0};
+    }
+  // fragments of half a step (int8 weights with bf16 rows: the raw bytes of the whole step
+  // are read with its first half)
+  struct Half {
+    bf16x8 a[MI];
+    bf16x8 w[NI];
+  };
+  auto read_a = [&](int s, int st, Half& f) {
+    const uint16_t* As = reinterpret_cast<const uint16_t*>(smem + (s % NS) * SS) + wm * MI * 16 * 64;
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+      f.a[m] = *reinterpret_cast<const bf16x8*>(As + a_at<kOrder>(m * 16 + c, KIND == kII ? 4 * st + q : 2 * q + st));
+  };
+  auto weights = [&](int s) { return smem + (s % NS) * SS + SA + wn * NI * BB + lane * 16; };
+  auto read_w = [&](int s, int st, Half& f) {
+    const uint8_t* Bs = weights(s) + st * 1024;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) f.w[n] = *reinterpret_cast<const bf16x8*>(Bs + n * BB);
+  };
+  auto multiply = [&](const Half& f) {
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
-        acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (KIND == kII) iacc[m][n] = int32x4{0, 0, 0, 0};
+        if constexpr (KIND == kII)
+          iacc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int32x4, f.w[n]),
+                                                             __builtin_bit_cast(int32x4, f.a[m]), iacc[m][n], 0, 0, 0);
+        else
+          acc[m][n] = mfma16(f.w[n], f.a[m], acc[m][n]);
       }
-    issue(0);
-    vm_barrier<0>();
-    for (int s = 0; s < steps; ++s) {
-      if (s + 1 < steps) issue(s + 1);
-      const uint16_t* As = reinterpret_cast<const uint16_t*>(smem + (s & 1) * (SA + SB)) + wm * MI * 16 * 64;
-      const uint8_t* Bs = smem + (s & 1) * (SA + SB) + SA + wn * NI * BB + lane * 16;
-      bf16x8 wf[2][NI];
-      if constexpr (KIND == kBI) {
+  };
+  // one read, then its share of the MFMAs, ...
+  auto interleave = [&] {
+    constexpr int R = MI + NI, M = MI * NI, each = M / R < 1 ? 1 : M / R;
 #pragma unroll
-        for (int n = 0; n < NI; ++n) cvt16(*reinterpret_cast<const uint4*>(Bs + n * BB), wf[0][n], wf[1][n]);
-      }
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        if constexpr (KIND != kBI) {
-#pragma unroll
-          for (int n = 0; n < NI; ++n) wf[st][n] = *reinterpret_cast<const bf16x8*>(Bs + n * BB + st * 1024);
-        }
-#pragma unroll
-        for (int m = 0; m < MI; ++m) {
-          const int r = m * 16 + c;
-          if constexpr (KIND == kII) {
-            const int32x4 a = *reinterpret_cast<const int32x4*>(As + a_at<0>(r, 4 * st + q));
-#pragma unroll
-            for (int n = 0; n < NI; ++n)
-              iacc[m][n] =
-                  __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int32x4, wf[st][n]), a, iacc[m][n], 0, 0, 0);
-          } else {
-            const bf16x8 a = *reinterpret_cast<const bf16x8*>(As + a_at<1>(r, 2 * q + st));
-#pragma unroll
-            for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(wf[st][n], a, acc[m][n]);
-          }
-        }
-      }
-      vm_barrier<0>();
+    for (int i = 0; i < R; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, each, 0);
     }
-    // scaled to f32
+    __builtin_amdgcn_sched_group_barrier(0x8, M, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const int steps = KIND == kII ? (p.kc + 1) >> 1 : p.kc;
 #pragma unroll
-    for (int m = 0; m < MI; ++m) {
-      float xs = 1.0f;
-      if constexpr (KIND == kII) {
-        const int pos = min(r0 + (wm * MI + m) * 16 + c, p.T - 1);
-        xs = p.xs[LORA ? p.order[pos] : pos];
+  for (int s = 0; s < NS; ++s)
+    if (s < steps) issue(s);
+  if (steps >= NS)
+    vm_barrier<(NS - 1) * PER>();
+  else
+    vm_barrier<0>();
+  Half f0, f1;
+  uint4 raw[KIND == kBI ? NI : 1];
+  auto read_first = [&](int s) {
+    read_a(s, 0, f0);
+    if constexpr (KIND == kBI) {
+#pragma unroll
+      for (int n = 0; n < NI; ++n) raw[n] = *reinterpret_cast<const uint4*>(weights(s) + n * BB);
+    } else {
+      read_w(s, 0, f0);
+    }
+  };
+  auto step = [&](int s, auto tail) {
+    read_a(s, 1, f1);
+    if constexpr (KIND == kBI) {
+#pragma unroll
+      for (int n = 0; n < NI; ++n) cvt16(raw[n], f0.w[n], f1.w[n]);
+    } else {
+      read_w(s, 1, f1);
+    }
+    multiply(f0);
+    interleave();
+    if constexpr (decltype(tail)::value) {
+      vm_barrier<0>();
+      if constexpr (LORA) {
+        // the adapters' first steps, while the last base steps run
+        if (next.at < rows) {
+          issue_lora(next, steps + issued++);
+          advance(next);
+        }
       }
+    } else {
+      vm_barrier<(NS - 2) * PER>();
+      issue(s + NS);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    read_first(s + 1);  // past the last step: what the stage holds, not used
+    multiply(f1);
+    interleave();
+  };
+  read_first(0);
+  int s = 0;
+  for (; s + NS < steps; ++s) step(s, std::false_type{});
+  for (; s < steps; ++s) step(s, std::true_type{});
+
+  // scaled to f32
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const int cg = min(cg0 + wn * NI + n, p.cgs - 1);
-        if constexpr (KIND == kII) {
-          const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + cg * 16 + 4 * q);
+  for (int m = 0; m < MI; ++m) {
+    float xs = 1.0f;
+    if constexpr (KIND == kII) {
+      const int r = (wm * MI + m) * 16 + c;
+      int row = min(r0 + r, p.T - 1);
+      if constexpr (LORA) row = seg[0][r];
+      xs = p.xs[row];
+    }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[m][n][j] = (float)iacc[m][n][j] * xs * sc[j];
-        } else if constexpr (KIND == kBI) {
-          const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + cg * 16 + 4 * q);
+    for (int n = 0; n < NI; ++n) {
+      const int cg = min(cg0 + wn * NI + n, p.cgs - 1);
+      if constexpr (KIND != kBB) {
+        const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + cg * 16 + 4 * q);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[m][n][j] *= sc[j];
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (KIND == kII)
+            acc[m][n][j] = (float)iacc[m][n][j] * xs * sc[j];
+          else
+            acc[m][n][j] *= sc[j];
         }
       }
     }
   }
   if constexpr (LORA) {
-    constexpr int LB = BN / 16 / NW;  // B loads per wave and step
-    const int rb = p.rp >> 5;
-    uint32_t uoff[AJ];
-#pragma unroll
-    for (int j = 0; j < AJ; ++j) {
-      const int r = 8 * (wv + NW * j) + (lane >> 3);
-      uoff[j] = (uint32_t)(min(r0 + r, p.T - 1) - r0) * (uint32_t)(rb * 128) +
-                (uint32_t)(a_piece_at<1>(r, lane & 7) * 16);
-    }
-    const char* ubase = reinterpret_cast<const char*>(p.u) + (size_t)r0 * rb * 128;
     const int w0 = wm * MI * 16;  // the wave's rows in the tile
-    for (int pos = r0; pos < r0 + rows;) {
-      const int ad = __builtin_amdgcn_readfirstlane(p.sorted[pos]);
-      if (ad < 0) break;
-      const int end = min(max(__builtin_amdgcn_readfirstlane(p.offsets[ad + 1]), pos + 1), r0 + rows);
-      const int lo = pos - r0, hi = end - r0;  // the adapter's rows in the tile
-      for (int s = 0; s < rb; ++s) {
+    for (; cur.at < rows; advance(cur), ++s) {
+      vm_barrier<0>();  // step s has landed, and every wave is done with the one before
+      if (next.at < rows && issued - (s - steps) < NS) {
+        issue_lora(next, steps + issued++);
+        advance(next);
+      }
+      const uint16_t* As = reinterpret_cast<const uint16_t*>(smem + (s % NS) * SS) + w0 * 64;
+      const uint8_t* Bs = smem + (s % NS) * SS + SA + wn * NI * 1024 + c * 16;
+      bf16x8 wf[2][NI];
 #pragma unroll
-        for (int j = 0; j < AJ; ++j) dma16(uoff[j], ubase + s * 128, lds0 + (wv + NW * j) * 1024);
+      for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int j = 0; j < LB; ++j) {
-          const int cg = min(cg0 + wv + NW * j, p.cgs - 1);
-          dma16(lane * 16, p.b + (((size_t)ad * p.cgs + cg) * rb + s) * 1024, lds0 + SA + (wv + NW * j) * 1024);
-        }
-        vm_barrier<0>();
-        const uint16_t* As = reinterpret_cast<const uint16_t*>(smem) + w0 * 64;
-        const uint8_t* Bs = smem + SA + wn * NI * 1024 + c * 16;
-        bf16x8 wf[2][NI];
+        for (int n = 0; n < NI; ++n)
+          wf[st][n] = *reinterpret_cast<const bf16x8*>(Bs + n * 1024 + (2 * (q & 1) + st) * 256);
 #pragma unroll
-        for (int st = 0; st < 2; ++st)
+      for (int m = 0; m < MI; ++m) {
+        const int g0 = w0 + m * 16;
+        if (g0 + 16 <= cur.at || g0 >= cur.end) continue;
+        const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(As + a_at<1>(m * 16 + c, 2 * q));
+        const bf16x8 a1 = *reinterpret_cast<const bf16x8*>(As + a_at<1>(m * 16 + c, 2 * q + 1));
+        if (g0 >= cur.at && g0 + 16 <= cur.end) {
 #pragma unroll
-          for (int n = 0; n < NI; ++n)
-            wf[st][n] = *reinterpret_cast<const bf16x8*>(Bs + n * 1024 + (2 * (q & 1) + st) * 256);
+          for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, acc[m][n]));
+        } else {
+          const bool mine = g0 + c >= cur.at && g0 + c < cur.end;
 #pragma unroll
-        for (int m = 0; m < MI; ++m) {
-          const int g0 = w0 + m * 16;
-          if (g0 + 16 <= lo || g0 >= hi) continue;
-          const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(As + a_at<1>(m * 16 + c, 2 * q));
-          const bf16x8 a1 = *reinterpret_cast<const bf16x8*>(As + a_at<1>(m * 16 + c, 2 * q + 1));
-          if (g0 >= lo && g0 + 16 <= hi) {
+          for (int n = 0; n < NI; ++n) {
+            const floatx4 t = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, floatx4{0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
-            for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, acc[m][n]));
-          } else {
-            const bool mine = g0 + c >= lo && g0 + c < hi;
-#pragma unroll
-            for (int n = 0; n < NI; ++n) {
-              const floatx4 t = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, floatx4{0.f, 0.f, 0.f, 0.f}));
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[m][n][j] = mine ? acc[m][n][j] + t[j] : acc[m][n][j];
-            }
+            for (int j = 0; j < 4; ++j) acc[m][n][j] = mine ? acc[m][n][j] + t[j] : acc[m][n][j];
           }
         }
-        vm_barrier<0>();
       }
-      pos = end;
     }
   }
   const bool vec = (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
 #pragma unroll
   for (int m = 0; m < MI; ++m) {
-    const int pos = r0 + (wm * MI + m) * 16 + c;
-    if (pos >= p.T) continue;
-    uint16_t* o = p.out + (size_t)(LORA ? p.order[pos] : pos) * p.N;
+    const int r = (wm * MI + m) * 16 + c;
+    if (r >= rows) continue;
+    int row = r0 + r;
+    if constexpr (LORA) row = seg[0][r];
+    uint16_t* o = p.out + (size_t)row * p.N;
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
       const int cg = cg0 + wn * NI + n;
@@ -695,45 +966,80 @@ dim3 grid_for(int64_t items) {
 }
 
 template <int KIND, int RB>
-void decode_of(const LinearArgs& p, hipStream_t st) {
-  hipLaunchKernelGGL((k_linear_decode<KIND, RB, 2>), dim3((p.cgs + 1) / 2), dim3(512), 0, st, p);
-}
-
-template <int KIND>
-void decode(const LinearArgs& p, hipStream_t st) {
-  switch ((p.T + 15) / 16) {
-    case 1:
-      return decode_of<KIND, 1>(p, st);
-    case 2:
-      return decode_of<KIND, 2>(p, st);
-    case 3:
-      return decode_of<KIND, 3>(p, st);
-    default:
-      return decode_of<KIND, 4>(p, st);
+void decode_of(const LinearArgs& p, bool split, hipStream_t st) {
+  // Adapters, or rows of more than 256 KB, which every block of the single launch reads whole:
+  // two launches. bf16 rows, int8 weights, us (single, two launches): 64 x 4096 -> 2048 18.4,
+  // 10.9; 64 x 8192 -> 4096 33.8, 23.6; but 64 x 2048 -> 5120 11.5, 12.4; 24 x 2048 -> 5120
+  // 6.6, 9.1; one row 2048 -> 5120 4.4, 6.8.
+  if (p.adapter || split) {
+    // eight waves of 16 columns share the rows' LDS reads less than four of 32, but convert
+    // and load beside more others: 24 rows of rank 64, 4096 -> 9216, 23.0 us on bf16 rows
+    // (four 28.9), on int8 rows, which take half the LDS and no conversion, 22.6 (four 19.5)
+    constexpr int NW = KIND == kII ? 4 : 8, CG = KIND == kII ? 2 : 1, ST = kSplitSteps;
+    const int steps = KIND == kII ? (p.kc + 1) / 2 : p.kc, splits = (steps + ST - 1) / ST;
+    const int blocks = (p.cgs + NW * CG - 1) / (NW * CG) * splits, shrink = p.adapter ? p.T * ((p.rank + 15) / 16) : 0;
+    hipLaunchKernelGGL((k_linear_split<KIND, RB, NW, CG>), dim3(shrink + blocks), dim3(64 * NW), 0, st, p, splits,
+                       shrink);
+    hipLaunchKernelGGL((k_linear_finish<KIND>), dim3((p.cgs * 4 + 63) / 64, p.T), dim3(64), 0, st, p, splits);
+  } else if (p.cgs <= 256) {
+    // one column group per block while that is no more than a block per CU (one row 8192 ->
+    // 4096 7.7 us, two groups 10.8); above, two, which share the rows (24 x 2048 -> 5120 6.6, one 8.9)
+    hipLaunchKernelGGL((k_linear_decode<KIND, RB, 1>), dim3(p.cgs), dim3(512), 0, st, p);
+  } else {
+    hipLaunchKernelGGL((k_linear_decode<KIND, RB, 2>), dim3((p.cgs + 1) / 2), dim3(512), 0, st, p);
   }
 }
 
-template <int KIND, int WM, int WN, int MI, int NI>
+template <int KIND>
+void decode(const LinearArgs& p, bool split, hipStream_t st) {
+  switch ((p.T + 15) / 16) {
+    case 1:
+      return decode_of<KIND, 1>(p, split, st);
+    case 2:
+      return decode_of<KIND, 2>(p, split, st);
+    case 3:
+      return decode_of<KIND, 3>(p, split, st);
+    default:
+      return decode_of<KIND, 4>(p, split, st);
+  }
+}
+
+template <int KIND, int WM, int WN, int MI, int NI, int NS>
 void gemm_of(const LinearArgs& p, hipStream_t st) {
   constexpr int BM = 16 * WM * MI, BN = 16 * WN * NI;
   const int tm = (p.T + BM - 1) / BM, tn = (p.cgs * 16 + BN - 1) / BN;
   const dim3 grid((unsigned)((((int64_t)tm * tn + 7) >> 3) * 8));
   if (p.adapter)
-    hipLaunchKernelGGL((k_linear_gemm<KIND, WM, WN, MI, NI, true>), grid, dim3(64 * WM * WN), 0, st, p, tm, tn);
+    hipLaunchKernelGGL((k_linear_gemm<KIND, WM, WN, MI, NI, NS, true>), grid, dim3(64 * WM * WN), 0, st, p, tm, tn);
   else
-    hipLaunchKernelGGL((k_linear_gemm<KIND, WM, WN, MI, NI, false>), grid, dim3(64 * WM * WN), 0, st, p, tm, tn);
+    hipLaunchKernelGGL((k_linear_gemm<KIND, WM, WN, MI, NI, NS, false>), grid, dim3(64 * WM * WN), 0, st, p, tm, tn);
 }
 
 template <int KIND>
-void linear_kind(const LinearArgs& p, hipStream_t st) {
-  if (p.T <= kLinearDecodeTokens) {
-    if (p.adapter)
-      hipLaunchKernelGGL((k_lora_shrink_rows<KIND>), dim3(p.T, (p.rank + 15) / 16), dim3(1024), 0, st, p);
-    decode<KIND>(p, st);
-    return;
-  }
-  if (p.adapter) hipLaunchKernelGGL((k_lora_shrink<KIND>), dim3((p.T + 15) / 16), dim3(512), 0, st, p);
-  gemm_of<KIND, 2, 2, 4, 4>(p, st);
+void gemm(const LinearArgs& p, hipStream_t st) {
+  const int64_t tiles = (int64_t)((p.T + 127) / 128) * ((p.cgs + 7) / 8);
+  if (tiles >= 256)
+    gemm_of<KIND, 2, 2, 4, 4, 2>(p, st);
+  else
+    gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
+}
+
+template <int KIND>
+void shrink(const LinearArgs& p, hipStream_t st) {
+  const dim3 grid((p.T + 15) / 16);
+  if (p.rank <= 16)
+    hipLaunchKernelGGL((k_lora_shrink<KIND, 1>), grid, dim3(1024), 0, st, p);
+  else if (p.rank <= 32)
+    hipLaunchKernelGGL((k_lora_shrink<KIND, 2>), grid, dim3(1024), 0, st, p);
+  else
+    hipLaunchKernelGGL((k_lora_shrink<KIND, 4>), grid, dim3(1024), 0, st, p);
+}
+
+template <int KIND>
+void linear_kind(const LinearArgs& p, bool split, hipStream_t st) {
+  if (p.T <= kLinearDecodeTokens) return decode<KIND>(p, split, st);
+  if (p.adapter) shrink<KIND>(p, st);
+  gemm<KIND>(p, st);
 }
 
 }  // namespace
@@ -817,12 +1123,14 @@ hipError_t launch_linear(const kmoe_linear_weight& w, int64_t tokens, const void
     p.kcp = Kp / 64;
     p.u = ws + space.u;
   }
+  p.part = reinterpret_cast<floatx4*>(ws + space.part);
+  const bool split = linear_splits(w, tokens, x_dtype);
   if (x_dtype == KMOE_DTYPE_I8)
-    linear_kind<kII>(p, st);
+    linear_kind<kII>(p, split, st);
   else if (w.dtype == KMOE_DTYPE_I8)
-    linear_kind<kBI>(p, st);
+    linear_kind<kBI>(p, split, st);
   else
-    linear_kind<kBB>(p, st);
+    linear_kind<kBB>(p, split, st);
   return hipGetLastError();
 }
 

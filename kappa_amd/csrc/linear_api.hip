@@ -55,6 +55,11 @@ kmoe_status kmoe_linear_workspace_bytes(const kmoe_linear_weight* w, int64_t tok
   return validate_linear_workspace_bytes(w, tokens, x_dtype, lora, bytes);
 }
 
+kmoe_status kmoe_linear_call_bytes(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                                   int64_t x_stride, const kmoe_lora* lora, size_t* bytes) {
+  return validate_linear_call_bytes(w, tokens, x, x_dtype, x_stride, lora, bytes);
+}
+
 kmoe_status kmoe_linear(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
                         int64_t x_stride, const float* x_scale, const kmoe_lora* lora, const kmoe_lora_batch* batch,
                         void* out, void* workspace, size_t workspace_bytes, void* stream) {

@@ -43,12 +43,30 @@ bool linear_rows_fit(const kmoe_linear_weight& w, const void* x, kmoe_dtype x_dt
          x_stride * (int64_t)dtype_size(x_dtype) % 16 == 0;
 }
 
-LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora) {
+bool linear_splits(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype) {
+  const int64_t chunks = (w.in_features + 63) / 64 * 64 * (int64_t)dtype_size(x_dtype);
+  return tokens > 0 && tokens <= kmoe::kLinearDecodeTokens && round_up(tokens, 16) * chunks > 256 * 1024;
+}
+
+LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora,
+                         bool copied) {
+  const size_t T = (size_t)tokens, in = (size_t)padded_in(w.in_features);
+  const bool splits = tokens <= kmoe::kLinearDecodeTokens && (lora || linear_splits(w, tokens, x_dtype));
+  const size_t parts = (in / (size_t)step_of(x_dtype) + kmoe::kSplitSteps - 1) / kmoe::kSplitSteps;
   LinearSpace s;
-  s.u = align256((size_t)tokens * (size_t)padded_in(w.in_features) * dtype_size(x_dtype));
+  s.part = copied ? align256(T * in * dtype_size(x_dtype)) : 0;
+  s.u = s.part + (splits ? align256(parts * T * (size_t)padded_out(w.out_features) * 4) : 0);
   // f32 per token and rank, or two bf16
-  s.total = s.u + (lora ? align256((size_t)tokens * (size_t)padded_rank(lora->rank) * 4) : 0);
+  s.total = s.u + (lora ? align256(T * (size_t)padded_rank(lora->rank) * 4) : 0);
   return s;
+}
+
+size_t linear_most_bytes(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora) {
+  const size_t own = linear_space(w, tokens, x_dtype, lora, true).total;
+  if (tokens <= kmoe::kLinearDecodeTokens) return own;
+  // just above the sizes that hold partial sums
+  const size_t below = linear_space(w, kmoe::kLinearDecodeTokens, x_dtype, lora, true).total;
+  return own > below ? own : below;
 }
 
 kmoe_status check_linear_weight(const kmoe_linear_weight* w, bool buffers) {
@@ -174,7 +192,15 @@ kmoe_status validate_linear_workspace_bytes(const kmoe_linear_weight* w, int64_t
     KMOE_TRY(check_beside(*w, *lora));
   }
   if (!bytes) return fail(KMOE_ERR_INVALID_ARG, "bytes is NULL");
-  *bytes = linear_space(*w, tokens, x_dtype, lora).total;
+  *bytes = linear_most_bytes(*w, tokens, x_dtype, lora);
+  return KMOE_OK;
+}
+
+kmoe_status validate_linear_call_bytes(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                                       int64_t x_stride, const kmoe_lora* lora, size_t* bytes) {
+  KMOE_TRY(validate_linear_workspace_bytes(w, tokens, x_dtype, lora, bytes));
+  if (x_stride < 0 || x_stride > kMostRowBytes) return fail(KMOE_ERR_INVALID_ARG, "x_stride %lld", (long long)x_stride);
+  *bytes = tokens > 0 ? linear_space(*w, tokens, x_dtype, lora, !linear_rows_fit(*w, x, x_dtype, x_stride)).total : 0;
   return KMOE_OK;
 }
 
@@ -206,8 +232,8 @@ kmoe_status validate_linear(const kmoe_linear_weight* w, int64_t tokens, const v
   if (tokens > 0 && (x_stride > kMostRowBytes || x_stride * size > row || padded_in(w->in_features) * size > row))
     return fail(KMOE_ERR_UNSUPPORTED, "x must span less than 4 GiB");
   if (tokens > 0 && (!x || !out)) return fail(KMOE_ERR_INVALID_ARG, "kmoe_linear: x and out must be non-NULL");
-  *space = linear_space(*w, tokens, x_dtype, lora);
-  if (tokens > 0 && (!workspace || workspace_bytes < space->total))
+  *space = linear_space(*w, tokens, x_dtype, lora, tokens > 0 && !linear_rows_fit(*w, x, x_dtype, x_stride));
+  if (tokens > 0 && ((!workspace && space->total > 0) || workspace_bytes < space->total))
     return fail(KMOE_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes is smaller than the %zu required",
                 workspace_bytes, space->total);
   if (tokens > 0 && !aligned16(workspace))

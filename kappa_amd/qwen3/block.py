@@ -19,7 +19,8 @@ import torch
 from .. import _lib
 from .architecture import Qwen3Config
 from .ffn_moe import PackedExperts, _desc, _impl_and_capacity, _moe_forward, _norm_scale, _stream
-from .projection import Q8Rows, _OnDevice
+from .projection import Q8Rows, _elsewhere
+from .projection import _stream as _raw_stream
 from .quant import Weight, kmoe_dtype
 
 
@@ -67,7 +68,12 @@ def _norm_inputs(x: torch.Tensor, residual: torch.Tensor | None, scale: torch.Te
             f"{getattr(residual, 'device', None)})"
         )
     d = int(x.shape[-1])
-    sc = _norm_scale(scale, d, x.device)
+    sc = scale
+    if not (
+        isinstance(sc, torch.Tensor) and sc.dim() == 1 and sc.numel() == d and sc.dtype == x.dtype
+        and sc.device == x.device and sc.is_contiguous()
+    ):  # fmt: skip
+        sc = _norm_scale(scale, d, x.device)
     return x.contiguous(), None if residual is None else residual.contiguous(), sc, x.numel() // d if d else 0, d
 
 
@@ -80,14 +86,17 @@ def add_rms_norm(
     x, residual, sc, T, d = _norm_inputs(x, residual, scale)
     if residual is None:
         raise ValueError("add_rms_norm needs a residual (rms_norm takes none)")
-    with _OnDevice(x.device):
-        h, out = torch.empty_like(x), torch.empty_like(x)
-        _lib.check(
-            _lib.lib().kmoe_add_rms_norm(
-                _desc(T, d, 1, 1, 1, x.dtype), x.data_ptr(), residual.data_ptr(), sc.data_ptr(), kmoe_dtype(sc.dtype),
-                float(epsilon), h.data_ptr(), out.data_ptr(), _stream(x.device),
-            )
-        )  # fmt: skip
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return add_rms_norm(x, residual, sc, epsilon=epsilon)
+    h, out = torch.empty_like(x), torch.empty_like(x)
+    _lib.check(
+        _lib.lib().kmoe_add_rms_norm(
+            _desc(T, d, 1, 1, 1, x.dtype), x.data_ptr(), residual.data_ptr(), sc.data_ptr(), kmoe_dtype(sc.dtype),
+            float(epsilon), h.data_ptr(), out.data_ptr(), _raw_stream(dev),
+        )
+    )  # fmt: skip
     return out, h
 
 
@@ -99,17 +108,20 @@ def add_rms_norm_q8(
     rint(v / rows.scale)``; a row with an infinity or a NaN has a NaN scale. ``residual`` may
     be None (``h`` is ``x``)."""
     x, residual, sc, T, d = _norm_inputs(x, residual, scale)
-    with _OnDevice(x.device):
-        h = x if residual is None else torch.empty_like(x)
-        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        s = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
-        _lib.check(
-            _lib.lib().kmoe_add_rms_norm_q8(
-                _desc(T, d, 1, 1, 1, x.dtype), x.data_ptr(), None if residual is None else residual.data_ptr(),
-                sc.data_ptr(), kmoe_dtype(sc.dtype), float(epsilon), None if residual is None else h.data_ptr(),
-                q.data_ptr(), s.data_ptr(), _stream(x.device),
-            )
-        )  # fmt: skip
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return add_rms_norm_q8(x, residual, sc, epsilon=epsilon)
+    h = x if residual is None else torch.empty_like(x)
+    q = torch.empty_like(x, dtype=torch.int8)
+    s = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=dev)
+    _lib.check(
+        _lib.lib().kmoe_add_rms_norm_q8(
+            _desc(T, d, 1, 1, 1, x.dtype), x.data_ptr(), None if residual is None else residual.data_ptr(),
+            sc.data_ptr(), kmoe_dtype(sc.dtype), float(epsilon), None if residual is None else h.data_ptr(),
+            q.data_ptr(), s.data_ptr(), _raw_stream(dev),
+        )
+    )  # fmt: skip
     return Q8Rows(q, s), h
 
 

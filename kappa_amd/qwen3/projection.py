@@ -36,24 +36,14 @@ class Q8Rows(NamedTuple):
     scale: torch.Tensor  # [..., 1] float32
 
 
-class _OnDevice:
-    """Makes a tensor's device the current one where it is not (launches go to the current device)."""
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.index is not None and self.index != self.before:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.index is not None and self.index != self.before:
-            torch.cuda.set_device(self.before)
-
-
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of ``device`` (the raw handle: a torch.cuda.Stream for it takes 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _elsewhere(device: torch.device) -> bool:
+    """Whether ``device`` is not the current one, where launches go."""
+    return device.index != torch.cuda.current_device()
 
 
 @dataclass(frozen=True)
@@ -88,7 +78,7 @@ def prepack_linear(w: Union[torch.Tensor, Q8Weight]) -> PackedLinear:
     nv, ns = ctypes.c_size_t(), ctypes.c_size_t()
     L = _lib.lib()
     _lib.check(L.kmoe_linear_pack_bytes(st, ctypes.byref(nv), ctypes.byref(ns)))
-    with _OnDevice(v.device):
+    with torch.cuda.device(v.device):
         src, keep = weight_struct(w, v.device, n_out=N, n_groups=None, name="w")
         values = torch.empty(nv.value // dtype.itemsize, dtype=dtype, device=v.device)
         scale = torch.empty(ns.value // 4, dtype=torch.float32, device=v.device)
@@ -152,7 +142,7 @@ class LoraAdapters:
         else:
             f = torch.full((count,), float(factor), dtype=torch.float32, device=dev)
         a, b = a.contiguous(), b.contiguous()
-        with _OnDevice(dev):
+        with torch.cuda.device(dev):
             _lib.check(
                 _lib.lib().kmoe_lora_pack(
                     self.struct, first, count, r, a.data_ptr(), b.data_ptr(), f.data_ptr(), _stream(dev)
@@ -198,7 +188,7 @@ def lora_batch(adapter: torch.Tensor, num_adapters: int) -> LoraBatch:
     L = _lib.lib()
     n = ctypes.c_size_t()
     _lib.check(L.kmoe_lora_sort_bytes(st, ctypes.byref(n)))
-    with _OnDevice(dev):
+    with torch.cuda.device(dev):
         buf = torch.empty(3 * T + num_adapters + 1 + n.value // 4, dtype=torch.int32, device=dev)
         p = buf.data_ptr()
         st.adapter, st.order, st.sorted, st.offsets = p, p + 4 * T, p + 8 * T, p + 12 * T
@@ -249,6 +239,7 @@ def linear(
         v = v.reshape(T, K)
         if v.stride(1) != 1 or v.stride(0) < K:
             v = v.contiguous()
+    stride = v.stride(0) if T > 1 else K
     if (lora is None) != (batch is None):
         raise ValueError("lora and batch come together")
     ls = bs = None
@@ -258,16 +249,18 @@ def linear(
         if lora.a.device != dev or batch.buffer.device != dev:
             raise ValueError(f"the adapters are on {lora.a.device}, the batch on {batch.buffer.device}, w on {dev}")
         ls, bs = lora.struct, batch.struct
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return linear(x, w, lora=lora, batch=batch)
     L = _lib.lib()
     n = ctypes.c_size_t()
-    _lib.check(L.kmoe_linear_workspace_bytes(w.struct, T, code, ls, ctypes.byref(n)))
-    with _OnDevice(dev):
-        out = torch.empty((*shape, w.out_features), dtype=torch.bfloat16, device=dev)
-        ws = torch.empty(max(n.value, 1), dtype=torch.uint8, device=dev)
-        _lib.check(
-            L.kmoe_linear(
-                w.struct, T, v.data_ptr(), code, v.stride(0) if T > 1 else K, xs, ls, bs, out.data_ptr(), ws.data_ptr(), n.value,
-                _stream(dev),
-            )
-        )  # fmt: skip
+    _lib.check(L.kmoe_linear_call_bytes(w.struct, T, v.data_ptr(), code, stride, ls, ctypes.byref(n)))
+    out = torch.empty((*shape, w.out_features), dtype=torch.bfloat16, device=dev)
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
+    _lib.check(
+        L.kmoe_linear(
+            w.struct, T, v.data_ptr(), code, stride, xs, ls, bs, out.data_ptr(),
+            None if ws is None else ws.data_ptr(), n.value, _stream(dev),
+        )
+    )  # fmt: skip
     return out

@@ -41,7 +41,7 @@ def _misaligned(t):
     return v
 
 
-SHAPES = [(1, 1), (3, 63), (2, 64), (5, 100), (1, 1024), (4, 2048), (257, 2048), (33, 2560), (1, 4096), (70, 4096), (9, 4095)]
+SHAPES = [(1003, 64), (1500, 1000), (2049, 512), (1, 1), (3, 63), (2, 64), (5, 100), (1, 1024), (4, 2048), (257, 2048), (33, 2560), (1, 4096), (70, 4096), (9, 4095)]
 
 
 @pytest.mark.parametrize("act", ["bf16", "f32"])

@@ -103,8 +103,10 @@ def test_add_rms_norm_q8_refusals(over, frag):
         (dict(out=None), _lib.ERR_INVALID_ARG, "non-NULL"),
         (dict(stride=1 << 29), _lib.ERR_UNSUPPORTED, "4 GiB"),
         (dict(stride=(1 << 63) - 1), _lib.ERR_UNSUPPORTED, "4 GiB"),
-        (dict(ws=None), _lib.ERR_WORKSPACE_TOO_SMALL, "workspace"),
-        (dict(n=16), _lib.ERR_WORKSPACE_TOO_SMALL, "workspace"),
+        (dict(ws=None, lora=lora(), batch=batch()), _lib.ERR_WORKSPACE_TOO_SMALL, "workspace"),
+        (dict(n=16, lora=lora(), batch=batch()), _lib.ERR_WORKSPACE_TOO_SMALL, "workspace"),
+        (dict(ws=None, stride=257), _lib.ERR_WORKSPACE_TOO_SMALL, "workspace"),
+        (dict(ws=None, x=P + 2), _lib.ERR_WORKSPACE_TOO_SMALL, "workspace"),
         (dict(ws=P + 4), _lib.ERR_INVALID_ARG, "16-byte"),
         (dict(lora=lora()), _lib.ERR_INVALID_ARG, "come together"),
         (dict(batch=batch()), _lib.ERR_INVALID_ARG, "come together"),
@@ -168,11 +170,21 @@ def test_sizes():
     assert (a.value, b.value) == (2 * 128 * 64, 4 * 64)
     assert L.kmoe_lora_pack_bytes(lora(L=3, R=8, K=100, N=33), a, b) == _lib.OK
     assert (a.value, b.value) == (3 * 2 * 128 * 32, 3 * 2 * 32 * 64)
-    before = 0
-    for T in (0, 1, 64, 65, 300, 4096):
-        assert L.kmoe_linear_workspace_bytes(lin(), T, BF, lora(), a) == _lib.OK
-        assert a.value >= max(before, T * (2 * 256 + 4 * 16))
-        before = a.value
+    for l in (None, lora(K=4096)):
+        before = 0
+        for T in (0, 1, 63, 64, 65, 66, 300, 4096):
+            w = lin(K=4096)
+            assert L.kmoe_linear_workspace_bytes(w, T, BF, l, a) == _lib.OK
+            assert a.value >= max(before, T * (2 * 4096 + (4 * 16 if l else 0)))
+            before = a.value
+            # what one call takes: nothing for aligned rows without adapters, but for partial sums
+            for x, stride in ((P, 4096), (P + 2, 4096), (P, 4100), (P, 4104)):
+                assert L.kmoe_linear_call_bytes(w, T, x, BF, stride, l, b) == _lib.OK
+                assert b.value <= a.value
+            assert L.kmoe_linear_call_bytes(w, T, P, BF, 4096, l, b) == _lib.OK
+            if l is None:
+                assert (b.value == 0) == (not 32 < T <= 64)
+    assert L.kmoe_linear_call_bytes(lin(), 4, P, BF, -1, None, b) == _lib.ERR_INVALID_ARG
 
 
 def test_python_layer_refuses_cpu_tensors():
