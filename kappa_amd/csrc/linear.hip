@@ -677,26 +677,28 @@ __global__ __launch_bounds__(64) void k_linear_finish(LinearArgs p, int splits) 
 // infinity times zero) reaches a row.
 // ---------------------------------------------------------------------------
 template <int KIND, int WM, int WN, int MI, int NI, int NS, bool LORA>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_linear_gemm(LinearArgs p, int tm, int tn) {
+struct GemmShape {
+  static constexpr int kThreads = 64 * WM * WN, kRows = 16 * WM * MI, kCols = 16 * WN * NI;
+  static constexpr int kStage = kRows * 128 + kCols / 16 * (KIND == kBI ? 1024 : 2048);
+  static constexpr int kLds = NS * kStage, kSeg = LORA ? 3 * kRows : 3;
+};
+
+// One tile: rows from r0 on and column groups from cg0 on, with smem of kLds bytes and seg of
+// kSeg ints (per tile row: token, adapter, where the adapter's rows end). Every thread of the
+// block calls it, once.
+template <int KIND, int WM, int WN, int MI, int NI, int NS, bool LORA>
+__device__ __forceinline__ void gemm_tile(const LinearArgs& p, uint8_t* smem, int* segs, int r0, int cg0) {
   constexpr int NW = WM * WN, BM = 16 * WM * MI, BN = 16 * WN * NI;
   constexpr int BB = KIND == kBI ? 1024 : 2048;  // weight bytes of a column group per step
   constexpr int SA = BM * 128, SB = BN / 16 * BB, SS = SA + SB;
   constexpr int AJ = BM / 8 / NW, BJ = SB / 1024 / NW, PER = AJ + BJ;
   static_assert(BM % (8 * NW) == 0 && SB % (1024 * NW) == 0 && BN / 16 % NW == 0, "whole loads per wave");
   constexpr int kOrder = KIND == kII ? 0 : 1;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[NS * SS];
-  __shared__ int seg[LORA ? 3 : 1][LORA ? BM : 1];  // per tile row: token, adapter, where the adapter's rows end
+  int (*const seg)[LORA ? BM : 1] = reinterpret_cast<int(*)[LORA ? BM : 1]>(segs);
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, q = lane >> 4;
   const int wm = wv / WN, wn = wv % WN;
-  const int ntiles = tm * tn, per = (ntiles + 7) >> 3;
-  const int L = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || L >= ntiles) return;
-  constexpr int GM = 8;
-  const int grp = L / (GM * tn), in = L - grp * GM * tn, gsz = min(tm - grp * GM, GM);
-  const int mt = grp * GM + in % gsz, nt = in / gsz;
-  const int r0 = mt * BM, rows = min(BM, p.T - r0);
-  const int cg0 = nt * (BN / 16);
+  const int rows = min(BM, p.T - r0);
   const uint32_t lds0 = lds_addr(smem);
   auto stage_at = [&](int s, int off) { return __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)((s % NS) * SS + off)); };
 
@@ -770,15 +772,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_linear_gemm(LinearArgs p, i
     cur = next;
   }
 
-  floatx4 acc[MI][NI];
-  int32x4 iacc[KIND == kII ? MI : 1][KIND == kII ? NI : 1];
+  floatx4 acc[MI][NI];  // kII: the bits of i32 sums until they are scaled
 #pragma unroll
   for (int m = 0; m < MI; ++m)
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (KIND == kII) iacc[m][n] = int32x4{0, 0, 0, 0};
-    }
+    for (int n = 0; n < NI; ++n) acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
   // fragments of half a step (int8 weights with bf16 rows: the raw bytes of the whole step
   // are read with its first half)
   struct Half {
@@ -803,8 +801,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_linear_gemm(LinearArgs p, i
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
         if constexpr (KIND == kII)
-          iacc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int32x4, f.w[n]),
-                                                             __builtin_bit_cast(int32x4, f.a[m]), iacc[m][n], 0, 0, 0);
+          acc[m][n] = __builtin_bit_cast(
+              floatx4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int32x4, f.w[n]),
+                                                             __builtin_bit_cast(int32x4, f.a[m]),
+                                                             __builtin_bit_cast(int32x4, acc[m][n]), 0, 0, 0));
         else
           acc[m][n] = mfma16(f.w[n], f.a[m], acc[m][n]);
       }
@@ -872,28 +872,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_linear_gemm(LinearArgs p, i
   for (; s + NS < steps; ++s) step(s, std::false_type{});
   for (; s < steps; ++s) step(s, std::true_type{});
 
-  // scaled to f32
+  // scaled to f32, row by row of the accumulators (all at once took 60 registers more)
+  if constexpr (KIND != kBB) {
+    floatx4 sc[NI];
 #pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    float xs = 1.0f;
-    if constexpr (KIND == kII) {
-      const int r = (wm * MI + m) * 16 + c;
-      int row = min(r0 + r, p.T - 1);
-      if constexpr (LORA) row = seg[0][r];
-      xs = p.xs[row];
-    }
+    for (int n = 0; n < NI; ++n)
+      sc[n] = *reinterpret_cast<const floatx4*>(p.ws + min(cg0 + wn * NI + n, p.cgs - 1) * 16 + 4 * q);
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      const int cg = min(cg0 + wn * NI + n, p.cgs - 1);
-      if constexpr (KIND != kBB) {
-        const floatx4 sc = *reinterpret_cast<const floatx4*>(p.ws + cg * 16 + 4 * q);
+    for (int m = 0; m < MI; ++m) {
+      float xs = 1.0f;
+      if constexpr (KIND == kII) {
+        const int r = (wm * MI + m) * 16 + c;
+        int row = min(r0 + r, p.T - 1);
+        if constexpr (LORA) row = seg[0][r];
+        xs = p.xs[row];
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (KIND == kII)
-            acc[m][n][j] = (float)iacc[m][n][j] * xs * sc[j];
-          else
-            acc[m][n][j] *= sc[j];
-        }
+      for (int n = 0; n < NI; ++n) {
+        if constexpr (KIND == kII)
+          acc[m][n] = __builtin_convertvector(__builtin_bit_cast(int32x4, acc[m][n]), floatx4) * xs * sc[n];
+        else
+          acc[m][n] *= sc[n];
       }
     }
   }
@@ -950,6 +949,56 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_linear_gemm(LinearArgs p, i
       store4(o, cg * 16 + 4 * q, p.N, vec, v);
     }
   }
+}
+
+// Tile L of tm x tn: groups of eight row tiles, row tiles fastest, so that the tiles that run
+// together on an XCD share rows and columns in its L2.
+__device__ __forceinline__ void tile_at(int L, int tm, int tn, int& mt, int& nt) {
+  constexpr int GM = 8;
+  const int grp = L / (GM * tn), in = L - grp * GM * tn, gsz = min(tm - grp * GM, GM);
+  mt = grp * GM + in % gsz;
+  nt = in / gsz;
+}
+
+// block i of n (a multiple of 8) as an index whose neighbours share an XCD
+__device__ __forceinline__ int xcd_order(int i, int n) { return (i & 7) * (n >> 3) + (i >> 3); }
+
+// Tiles of one size.
+template <int KIND, int WM, int WN, int MI, int NI, int NS, bool LORA>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_linear_gemm(LinearArgs p, int tm, int tn) {
+  using Sh = GemmShape<KIND, WM, WN, MI, NI, NS, LORA>;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[Sh::kLds];
+  __shared__ int seg[Sh::kSeg];
+  const int L = xcd_order(blockIdx.x, gridDim.x);
+  if (L >= tm * tn) return;
+  int mt, nt;
+  tile_at(L, tm, tn, mt, nt);
+  gemm_tile<KIND, WM, WN, MI, NI, NS, LORA>(p, smem, seg, mt * Sh::kRows, nt * (Sh::kCols / 16));
+}
+
+// Many tiles: the first `whole` of 256 x 256, one per CU and round; the rest as quarters of
+// 128 x 128, so that the last round is a short one.
+template <int KIND, bool LORA>
+__global__ __launch_bounds__(512, 2) void k_linear_gemm_mixed(LinearArgs p, int tm, int tn, int whole) {
+  using Big = GemmShape<KIND, 2, 4, 8, 4, 2, LORA>;
+  using Small = GemmShape<KIND, 2, 4, 4, 2, 4, LORA>;
+  static_assert(Big::kThreads == Small::kThreads && Small::kLds <= Big::kLds && Small::kSeg <= Big::kSeg, "one block");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[Big::kLds];
+  __shared__ int seg[Big::kSeg];
+  int mt, nt;
+  if ((int)blockIdx.x < whole) {
+    const int L = xcd_order(blockIdx.x, whole);
+    if (L >= tm * tn) return;
+    tile_at(L, tm, tn, mt, nt);
+    gemm_tile<KIND, 2, 4, 8, 4, 2, LORA>(p, smem, seg, mt * 256, nt * 16);
+    return;
+  }
+  const int i = xcd_order(blockIdx.x - whole, gridDim.x - whole), L = whole + (i >> 2);
+  if (L >= tm * tn) return;
+  tile_at(L, tm, tn, mt, nt);
+  const int r0 = mt * 256 + (i & 1) * 128, cg0 = nt * 16 + (i >> 1 & 1) * 8;
+  if (r0 >= p.T || cg0 >= p.cgs) return;
+  gemm_tile<KIND, 2, 4, 4, 2, 4, LORA>(p, smem, seg, r0, cg0);
 }
 
 }  // namespace kmoe
@@ -1017,8 +1066,20 @@ void gemm_of(const LinearArgs& p, hipStream_t st) {
 
 template <int KIND>
 void gemm(const LinearArgs& p, hipStream_t st) {
-  const int64_t tiles = (int64_t)((p.T + 127) / 128) * ((p.cgs + 7) / 8);
-  if (tiles >= 256)
+  const int tm = (p.T + 255) / 256, tn = (p.cgs + 15) / 16;
+  const int64_t tiles = (int64_t)tm * tn;
+  if (tiles >= 256) {
+    // what is left after the whole rounds goes in quarters unless those would take four rounds
+    const int64_t rest = tiles % 256, whole = rest > 192 ? (tiles + 7) / 8 * 8 : tiles - rest;
+    const int64_t blocks = rest > 192 ? whole : whole + (4 * rest + 7) / 8 * 8;
+    if (p.adapter)
+      hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, true>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn, (int)whole);
+    else
+      hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, false>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn, (int)whole);
+    return;
+  }
+  const int64_t mid = (int64_t)((p.T + 127) / 128) * ((p.cgs + 7) / 8);
+  if (mid >= 256)
     gemm_of<KIND, 2, 2, 4, 4, 2>(p, st);
   else
     gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
