@@ -1064,25 +1064,42 @@ void gemm_of(const LinearArgs& p, hipStream_t st) {
     hipLaunchKernelGGL((k_linear_gemm<KIND, WM, WN, MI, NI, NS, false>), grid, dim3(64 * WM * WN), 0, st, p, tm, tn);
 }
 
+// The tile by how many there are, against 256 CUs. Times in us of tiles of 32 x 64, 64 x 64,
+// 64 x 128, 128 x 128 and 256 x 256, for n tiles of 128 x 128 (m of 256 x 256):
+//   1024 -> 512, 1024 rows (n = 32)       bf16 x int8  6.2   6.9   9.5  13.3  28.4
+//   4096 -> 2048, 333 rows (48)           bf16 x int8 19.6  18.5  26.9  39.3  83.6
+//   2560 -> 6144, 256 / 333 (96, 144)     bf16        20.9 / 29.3, 18.6 / 28.0, 17.5 / 25.5, 27.4 / 27.8
+//   4096 -> 2048, 1500 (192)              bf16 x int8 46.6  36.0  41.4  41.3  84.3
+//   2048 -> 5120, 700 (240)               bf16 x int8 28.8  26.1  23.9  24.5  48.8
+//   4096 -> 9216, 333 / 512 (216, 288)    int8        32.7 / 42.6, 28.0 / 38.4, 23.6 / 34.3, 24.9 / 33.6
+//   2048 -> 5120, 1500 (480)              bf16        63.7  53.0  43.7  36.7  51.2
+//   2048 -> 5120, 2048 (640; m = 160)     bf16 x int8 74.6  59.8  51.3  50.0  55.3
+//   2560 -> 6144, 2048 (768; m = 192)     bf16       119.7 101.2  77.9  72.0  64.2
+//   4096 -> 9216, 2048 (1152; m = 288)    int8       153.3 122.6  98.3  92.6  75.6 (quarters in the last round)
 template <int KIND>
 void gemm(const LinearArgs& p, hipStream_t st) {
   const int tm = (p.T + 255) / 256, tn = (p.cgs + 15) / 16;
-  const int64_t tiles = (int64_t)tm * tn;
-  if (tiles >= 256) {
-    // what is left after the whole rounds goes in quarters unless those would take four rounds
-    const int64_t rest = tiles % 256, whole = rest > 192 ? (tiles + 7) / 8 * 8 : tiles - rest;
-    const int64_t blocks = rest > 192 ? whole : whole + (4 * rest + 7) / 8 * 8;
+  const int64_t big = (int64_t)tm * tn, mid = (int64_t)((p.T + 127) / 128) * ((p.cgs + 7) / 8);
+  if (big >= 176) {
+    // what is left after the whole rounds goes in quarters, unless those would take four rounds
+    const int64_t rest = big % 256;
+    const bool quarters = big > 256 && rest <= 192;
+    const int64_t whole = quarters ? big - rest : (big + 7) / 8 * 8, blocks = whole + (quarters ? (4 * rest + 7) / 8 * 8 : 0);
     if (p.adapter)
-      hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, true>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn, (int)whole);
+      hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, true>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn,
+                         (int)whole);
     else
-      hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, false>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn, (int)whole);
-    return;
-  }
-  const int64_t mid = (int64_t)((p.T + 127) / 128) * ((p.cgs + 7) / 8);
-  if (mid >= 256)
+      hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, false>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn,
+                         (int)whole);
+  } else if (mid >= 256) {
     gemm_of<KIND, 2, 2, 4, 4, 2>(p, st);
-  else
+  } else if (mid >= (KIND == kBI ? 224 : 144)) {
+    gemm_of<KIND, 1, 4, 4, 2, 3>(p, st);
+  } else if (mid > 32) {
     gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
+  } else {
+    gemm_of<KIND, 1, 4, 2, 1, 4>(p, st);
+  }
 }
 
 template <int KIND>

@@ -8,7 +8,7 @@ namespace {
 
 constexpr int64_t kMostIn = (int64_t)1 << 16;  // int8 sums stay inside i32
 constexpr int64_t kMostOut = (int64_t)1 << 20;
-constexpr int64_t kMostTokens = (int64_t)1 << 24;
+constexpr int64_t kMostTokens = (int64_t)1 << 20;  // the sort's blocks read each other's counts
 constexpr int64_t kMostRowBytes = (int64_t)1 << 32;  // 32-bit load offsets
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }

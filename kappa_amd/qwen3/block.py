@@ -50,31 +50,39 @@ def rms_norm(
     return out.reshape(x.shape)
 
 
+_CODE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+
+
 def _norm_inputs(x: torch.Tensor, residual: torch.Tensor | None, scale: torch.Tensor):
-    """Flattened contiguous x and residual, the norm scale, T and D."""
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
+    """Contiguous x and residual, the norm scale, and kmoe_desc (the checks a serving loop pays
+    for on every call are kept to attributes)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"x must be a torch tensor on a HIP device (got {getattr(x, 'device', type(x))})")
-    if x.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"x must be bfloat16 or float32 (got {x.dtype})")
-    if x.dim() < 1:
+    dtype, dev, shape = x.dtype, x.device, x.shape
+    code = _CODE.get(dtype)
+    if code is None:
+        raise ValueError(f"x must be bfloat16 or float32 (got {dtype})")
+    if not shape:
         raise ValueError("x must have at least one axis")
-    if residual is not None and (
-        not isinstance(residual, torch.Tensor)
-        or residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device
-    ):  # fmt: skip
-        raise ValueError(
-            f"residual must be as x, {tuple(x.shape)} {x.dtype} on {x.device} (got "
-            f"{tuple(getattr(residual, 'shape', ()))} {getattr(residual, 'dtype', type(residual))} on "
-            f"{getattr(residual, 'device', None)})"
-        )
-    d = int(x.shape[-1])
-    sc = scale
+    if residual is not None:
+        if (
+            not isinstance(residual, torch.Tensor)
+            or residual.shape != shape or residual.dtype != dtype or residual.device != dev
+        ):  # fmt: skip
+            raise ValueError(
+                f"residual must be as x, {tuple(shape)} {dtype} on {dev} (got "
+                f"{tuple(getattr(residual, 'shape', ()))} {getattr(residual, 'dtype', type(residual))} on "
+                f"{getattr(residual, 'device', None)})"
+            )
+        residual = residual.contiguous()
+    d = shape[-1]
     if not (
-        isinstance(sc, torch.Tensor) and sc.dim() == 1 and sc.numel() == d and sc.dtype == x.dtype
-        and sc.device == x.device and sc.is_contiguous()
+        isinstance(scale, torch.Tensor) and scale.shape == shape[-1:] and scale.dtype in _CODE
+        and scale.device == dev and scale.is_contiguous()
     ):  # fmt: skip
-        sc = _norm_scale(scale, d, x.device)
-    return x.contiguous(), None if residual is None else residual.contiguous(), sc, x.numel() // d if d else 0, d
+        scale = _norm_scale(scale, d, dev)
+    desc = _lib.KmoeDesc(x.numel() // d if d else 0, d, 1, 1, 1, code, _lib.IMPL_GATHER_EINSUM, 64, 0, _lib.KERNELS_AUTO)
+    return x.contiguous(), residual, scale, desc
 
 
 def add_rms_norm(
@@ -83,9 +91,9 @@ def add_rms_norm(
     """The residual's addition and the norm after it, in one pass: ``(rms_norm(h, scale), h)``
     with ``h = x + residual`` (kappa/qwen3/block.py:71, 153, 196), bit for bit what the two
     steps give. ``x`` and ``residual`` are ``[..., D]`` of one type, bfloat16 or float32."""
-    x, residual, sc, T, d = _norm_inputs(x, residual, scale)
     if residual is None:
         raise ValueError("add_rms_norm needs a residual (rms_norm takes none)")
+    x, residual, sc, desc = _norm_inputs(x, residual, scale)
     dev = x.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
@@ -93,8 +101,8 @@ def add_rms_norm(
     h, out = torch.empty_like(x), torch.empty_like(x)
     _lib.check(
         _lib.lib().kmoe_add_rms_norm(
-            _desc(T, d, 1, 1, 1, x.dtype), x.data_ptr(), residual.data_ptr(), sc.data_ptr(), kmoe_dtype(sc.dtype),
-            float(epsilon), h.data_ptr(), out.data_ptr(), _raw_stream(dev),
+            desc, x.data_ptr(), residual.data_ptr(), sc.data_ptr(), _CODE[sc.dtype], float(epsilon), h.data_ptr(),
+            out.data_ptr(), _raw_stream(dev),
         )
     )  # fmt: skip
     return out, h
@@ -107,7 +115,7 @@ def add_rms_norm_q8(
     ``v`` the normalised row in float32, ``rows.scale = max|v| / 127`` and ``rows.values =
     rint(v / rows.scale)``; a row with an infinity or a NaN has a NaN scale. ``residual`` may
     be None (``h`` is ``x``)."""
-    x, residual, sc, T, d = _norm_inputs(x, residual, scale)
+    x, residual, sc, desc = _norm_inputs(x, residual, scale)
     dev = x.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
@@ -117,9 +125,8 @@ def add_rms_norm_q8(
     s = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=dev)
     _lib.check(
         _lib.lib().kmoe_add_rms_norm_q8(
-            _desc(T, d, 1, 1, 1, x.dtype), x.data_ptr(), None if residual is None else residual.data_ptr(),
-            sc.data_ptr(), kmoe_dtype(sc.dtype), float(epsilon), None if residual is None else h.data_ptr(),
-            q.data_ptr(), s.data_ptr(), _raw_stream(dev),
+            desc, x.data_ptr(), None if residual is None else residual.data_ptr(), sc.data_ptr(), _CODE[sc.dtype],
+            float(epsilon), None if residual is None else h.data_ptr(), q.data_ptr(), s.data_ptr(), _raw_stream(dev),
         )
     )  # fmt: skip
     return Q8Rows(q, s), h

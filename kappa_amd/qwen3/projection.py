@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from functools import cached_property
 from typing import NamedTuple, Union
 
 import torch
@@ -43,18 +44,33 @@ def _stream(device: torch.device) -> int:
 
 def _elsewhere(device: torch.device) -> bool:
     """Whether ``device`` is not the current one, where launches go."""
-    return device.index != torch.cuda.current_device()
+    return device.index != torch._C._cuda_getDevice()
+
+
+class _WithStruct:
+    """Keeps the C struct of a frozen dataclass after its first use; copies make their own."""
+
+    def __getstate__(self):
+        state = dict(self.__dict__)
+        state.pop("struct", None)
+        return state
 
 
 @dataclass(frozen=True)
-class PackedLinear:
+class PackedLinear(_WithStruct):
     """A projection's weights in the gfx950 layout (include/kmoe.h, kmoe_linear_weight)."""
 
     values: torch.Tensor
     scale: torch.Tensor
     in_features: int
     out_features: int
-    struct: _lib.KmoeLinear
+
+    @cached_property
+    def struct(self) -> _lib.KmoeLinear:
+        code = _lib.DTYPE_I8 if self.values.dtype == torch.int8 else _lib.DTYPE_BF16
+        return _lib.KmoeLinear(
+            self.values.data_ptr(), self.scale.data_ptr(), code, self.in_features, self.out_features
+        )
 
     @property
     def nbytes(self) -> int:
@@ -82,13 +98,13 @@ def prepack_linear(w: Union[torch.Tensor, Q8Weight]) -> PackedLinear:
         src, keep = weight_struct(w, v.device, n_out=N, n_groups=None, name="w")
         values = torch.empty(nv.value // dtype.itemsize, dtype=dtype, device=v.device)
         scale = torch.empty(ns.value // 4, dtype=torch.float32, device=v.device)
-        st.values, st.scale = values.data_ptr(), scale.data_ptr()
-        _lib.check(L.kmoe_linear_pack(src, st, _stream(v.device)))
-    return PackedLinear(values, scale, K, N, st)
+        packed = PackedLinear(values, scale, K, N)
+        _lib.check(L.kmoe_linear_pack(src, packed.struct, _stream(v.device)))
+    return packed
 
 
 @dataclass(frozen=True)
-class LoraAdapters:
+class LoraAdapters(_WithStruct):
     """The adapters of one projection in the gfx950 layout (include/kmoe.h, kmoe_lora)."""
 
     a: torch.Tensor
@@ -98,7 +114,13 @@ class LoraAdapters:
     rank: int
     in_features: int
     out_features: int
-    struct: _lib.KmoeLora
+
+    @cached_property
+    def struct(self) -> _lib.KmoeLora:
+        return _lib.KmoeLora(
+            self.a.data_ptr(), self.b.data_ptr(), self.factor.data_ptr(), self.num_adapters, self.rank,
+            self.in_features, self.out_features,
+        )  # fmt: skip
 
     @staticmethod
     def empty(
@@ -114,8 +136,7 @@ class LoraAdapters:
         a = torch.zeros(na.value // 2, dtype=torch.bfloat16, device=device)
         b = torch.zeros(nb.value // 2, dtype=torch.bfloat16, device=device)
         factor = torch.zeros(num_adapters, dtype=torch.float32, device=device)
-        st.a, st.b, st.factor = a.data_ptr(), b.data_ptr(), factor.data_ptr()
-        return LoraAdapters(a, b, factor, num_adapters, rank, in_features, out_features, st)
+        return LoraAdapters(a, b, factor, num_adapters, rank, in_features, out_features)
 
     def store(self, first: int, a: torch.Tensor, b: torch.Tensor, factor: Union[float, torch.Tensor]) -> None:
         """Fills the slots ``first ..`` from ``a`` ``[count, in, r]`` and ``b`` ``[count, r, out]``
@@ -165,13 +186,17 @@ def prepack_lora(a: torch.Tensor, b: torch.Tensor, factor: Union[float, torch.Te
 
 
 @dataclass(frozen=True)
-class LoraBatch:
+class LoraBatch(_WithStruct):
     """A step's tokens sorted by adapter (include/kmoe.h, kmoe_lora_batch)."""
 
-    buffer: torch.Tensor
+    buffer: torch.Tensor  # int32: adapter, order and sorted [tokens], offsets [num_adapters + 1], the sort's scratch
     tokens: int
     num_adapters: int
-    struct: _lib.KmoeLoraBatch
+
+    @cached_property
+    def struct(self) -> _lib.KmoeLoraBatch:
+        p, n = self.buffer.data_ptr(), 4 * self.tokens
+        return _lib.KmoeLoraBatch(p, p + n, p + 2 * n, p + 3 * n, self.tokens, self.num_adapters)
 
 
 def lora_batch(adapter: torch.Tensor, num_adapters: int) -> LoraBatch:
@@ -190,10 +215,10 @@ def lora_batch(adapter: torch.Tensor, num_adapters: int) -> LoraBatch:
     _lib.check(L.kmoe_lora_sort_bytes(st, ctypes.byref(n)))
     with torch.cuda.device(dev):
         buf = torch.empty(3 * T + num_adapters + 1 + n.value // 4, dtype=torch.int32, device=dev)
-        p = buf.data_ptr()
-        st.adapter, st.order, st.sorted, st.offsets = p, p + 4 * T, p + 8 * T, p + 12 * T
-        _lib.check(L.kmoe_lora_sort(adapter.data_ptr(), st, p + 4 * (3 * T + num_adapters + 1), n.value, _stream(dev)))
-    return LoraBatch(buf, T, num_adapters, st)
+        batch = LoraBatch(buf, T, num_adapters)
+        scratch = buf.data_ptr() + 4 * (3 * T + num_adapters + 1)
+        _lib.check(L.kmoe_lora_sort(adapter.data_ptr(), batch.struct, scratch, n.value, _stream(dev)))
+    return batch
 
 
 def linear(

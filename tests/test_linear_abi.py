@@ -144,7 +144,7 @@ def test_packing_refusals():
     assert L.kmoe_lora_sort(None, batch(), P, 1 << 20, None) == _lib.ERR_INVALID_ARG
     assert L.kmoe_lora_sort(P, batch(), P, 19, None) == _lib.ERR_WORKSPACE_TOO_SMALL
     assert L.kmoe_lora_sort(P, batch(L=0), P, 1 << 20, None) == _lib.ERR_INVALID_ARG
-    assert L.kmoe_lora_sort(P, batch(T=(1 << 24) + 1), P, 1 << 40, None) == _lib.ERR_UNSUPPORTED
+    assert L.kmoe_lora_sort(P, batch(T=(1 << 20) + 1), P, 1 << 40, None) == _lib.ERR_UNSUPPORTED
 
 
 @NO_DEVICE
