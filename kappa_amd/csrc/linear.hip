@@ -1066,16 +1066,20 @@ void gemm_of(const LinearArgs& p, hipStream_t st) {
 
 // The tile by how many there are, against 256 CUs. Times in us of tiles of 32 x 64, 64 x 64,
 // 64 x 128, 128 x 128 and 256 x 256, for n tiles of 128 x 128 (m of 256 x 256):
-//   1024 -> 512, 1024 rows (n = 32)       bf16 x int8  6.2   6.9   9.5  13.3  28.4
-//   4096 -> 2048, 333 rows (48)           bf16 x int8 19.6  18.5  26.9  39.3  83.6
-//   2560 -> 6144, 256 / 333 (96, 144)     bf16        20.9 / 29.3, 18.6 / 28.0, 17.5 / 25.5, 27.4 / 27.8
-//   4096 -> 2048, 1500 (192)              bf16 x int8 46.6  36.0  41.4  41.3  84.3
-//   2048 -> 5120, 700 (240)               bf16 x int8 28.8  26.1  23.9  24.5  48.8
-//   4096 -> 9216, 333 / 512 (216, 288)    int8        32.7 / 42.6, 28.0 / 38.4, 23.6 / 34.3, 24.9 / 33.6
-//   2048 -> 5120, 1500 (480)              bf16        63.7  53.0  43.7  36.7  51.2
-//   2048 -> 5120, 2048 (640; m = 160)     bf16 x int8 74.6  59.8  51.3  50.0  55.3
-//   2560 -> 6144, 2048 (768; m = 192)     bf16       119.7 101.2  77.9  72.0  64.2
-//   4096 -> 9216, 2048 (1152; m = 288)    int8       153.3 122.6  98.3  92.6  75.6 (quarters in the last round)
+//   1024 -> 512, 1024 rows (n = 32)  bf16 x int8   6.2   7.4   9.9  13.8  28.4
+//   4096 -> 2048, 333 (48)           bf16 x int8  19.6  18.6  26.8  39.3  83.6
+//   2560 -> 6144, 200 / 512 (96, 192)       bf16  19.7 / 35.5, 16.4 / 26.6, 23.0 / 25.3, 27.5 / 28.0
+//   4096 -> 2048, 1500 (192)         bf16 x int8  46.6  34.5  37.2  39.9  84.3
+//   2048 -> 5120, 700 (240)          bf16 x int8  28.8  25.2  22.5  24.6  48.8
+//   4096 -> 9216, 333 / 512 (216, 288)      int8  32.7 / 42.6, 26.2 / 33.3, 22.0 / 29.3, 25.3 / 33.3
+//   2560 -> 6144, 1024 (384)                bf16  62.3  48.6  39.4  40.3  59.3
+//   2048 -> 5120, 1500 (480)                bf16  63.7  47.9  43.0  34.7  51.2
+//   2048 -> 5120, 2048 (640; m = 160) bf16 x int8 74.6  55.5  47.9  48.6  55.3
+//   2560 -> 6144, 2048 (768; m = 192)       bf16 119.7  93.6  74.2  70.1  64.2
+//   4096 -> 9216, 2048 (1152; m = 288)      int8 153.3 111.7  90.2  87.6  75.6 (quarters in the last round)
+// The smaller tiles are bound by LDS reads, so their four waves stand 2 x 2; int8 weights with
+// bf16 rows, which each wave converts for itself, want them 1 x 4 (64 x 64: 2048 -> 5120, 512
+// rows 19.0 against 21.3, bf16 weights 22.8 against 22.0).
 template <int KIND>
 void gemm(const LinearArgs& p, hipStream_t st) {
   const int tm = (p.T + 255) / 256, tn = (p.cgs + 15) / 16;
@@ -1091,12 +1095,18 @@ void gemm(const LinearArgs& p, hipStream_t st) {
     else
       hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, false>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn,
                          (int)whole);
-  } else if (mid >= 256) {
+  } else if (mid >= 400) {
     gemm_of<KIND, 2, 2, 4, 4, 2>(p, st);
   } else if (mid >= (KIND == kBI ? 224 : 144)) {
-    gemm_of<KIND, 1, 4, 4, 2, 3>(p, st);
+    if constexpr (KIND == kBI)
+      gemm_of<KIND, 1, 4, 4, 2, 3>(p, st);
+    else
+      gemm_of<KIND, 2, 2, 2, 4, 2>(p, st);
   } else if (mid > 32) {
-    gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
+    if constexpr (KIND == kBI)
+      gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
+    else
+      gemm_of<KIND, 2, 2, 2, 2, 4>(p, st);
   } else {
     gemm_of<KIND, 1, 4, 2, 1, 4>(p, st);
   }

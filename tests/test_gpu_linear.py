@@ -107,7 +107,8 @@ def test_linear(dev, T, K, N, weights, rows):
 
 
 # every tile of the GEMM, with rows and columns that end inside one
-TILES = [(513, 192, 500), (1100, 128, 2100), (1900, 64, 2000), (2100, 128, 2001), (3000, 192, 3900), (4200, 128, 4001),
+TILES = [(513, 192, 500), (1100, 128, 2100), (1900, 64, 2000), (2100, 128, 2001),
+         (2900, 64, 2400), (3000, 192, 3900), (4200, 128, 4001),
          (5400, 64, 5290)]  # fmt: skip
 
 
