@@ -9,6 +9,7 @@
 // Three kinds of products (Kind): bf16 rows with bf16 or int8 weights on
 // v_mfma_f32_16x16x32_bf16 (int8 becomes bf16 in registers, exactly), and int8 rows
 // with int8 weights on v_mfma_i32_16x16x64_i8, whose sums are exact.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -294,8 +295,9 @@ __device__ __forceinline__ void shrink_row(const LinearArgs& p, int t, int g, fl
 }
 
 // ---------------------------------------------------------------------------
-// u for many tokens, 16 sorted rows per block: MFMA, sixteen waves over the chunks, one
-// pass per adapter of the tile and NG groups of 16 ranks; u as bf16 hi + lo. Bound by
+// u for many tokens, 16 sorted rows per tile: MFMA, sixteen waves over the chunks, one
+// pass per adapter of the tile and NG groups of 16 ranks; u as bf16 hi + lo. The passes are
+// shared out over the blocks of the tile (y: the adapters, z: the groups). Bound by
 // latency: the tile's adapters come with its rows, and all chunks of 4096 elements are in
 // flight together.
 // ---------------------------------------------------------------------------
@@ -309,6 +311,14 @@ __global__ __launch_bounds__(1024) void k_lora_shrink(LinearArgs p) {
   const int r0 = blockIdx.x * 16, at = min(r0 + c, p.T - 1);
   const int row = p.order[at];
   const int mine = r0 + c < p.T ? p.sorted[at] : -1;
+  uint64_t left = __ballot(mine >= 0);  // the tile's rows whose adapter is still to come
+  auto first = [&] { return __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)left) - 1); };
+  // to the block's next adapter, gridDim.y further on
+  auto skip = [&](int k) {
+    for (; k > 0 && left; --k) left &= ~__ballot(mine == first());
+  };
+  skip(blockIdx.y);
+  if (!left) return;
   const char* const xr = p.x + (size_t)row * p.row_bytes + q * (16 * XL);
   const float xs = KIND == kII ? p.xs[row] : 1.0f;
   const int groups = (p.rank + 15) >> 4;
@@ -325,11 +335,8 @@ __global__ __launch_bounds__(1024) void k_lora_shrink(LinearArgs p) {
   // up to NW * CB chunks the rows stay in registers for every adapter and group
   const bool once = p.kc <= NW * CB;
   load_x(wv);
-  uint64_t left = __ballot(mine >= 0);  // the tile's rows whose adapter is still to come
-  while (left) {
-    const int ad = __shfl(mine, __ffsll((unsigned long long)left) - 1, 64);
-    const uint64_t these = __ballot(mine == ad);
-    left &= ~these;
+  for (; left; skip(gridDim.y)) {
+    const int ad = first();
     const float f = p.factor[ad] * xs;
     uint16_t* const u = reinterpret_cast<uint16_t*>(p.u) + (size_t)(r0 + c) * p.rp * 2;
     // ranks r .. r + 3 of this lane's row
@@ -341,7 +348,7 @@ __global__ __launch_bounds__(1024) void k_lora_shrink(LinearArgs p) {
       *reinterpret_cast<uint2*>(d) = uint2{hi[0] | (uint32_t)hi[1] << 16, hi[2] | (uint32_t)hi[3] << 16};
       *reinterpret_cast<uint2*>(d + 32) = uint2{lo[0] | (uint32_t)lo[1] << 16, lo[2] | (uint32_t)lo[3] << 16};
     };
-    for (int g0 = 0; g0 < groups; g0 += NG) {
+    for (int g0 = blockIdx.z * NG; g0 < groups; g0 += gridDim.z * NG) {
       const char* ar = p.a + (size_t)ad * p.rp * p.kcp * 128 + (size_t)g0 * p.kcp * 2048 + lane * 16;
       floatx4 acc[NG];
 #pragma unroll
@@ -390,7 +397,7 @@ __global__ __launch_bounds__(1024) void k_lora_shrink(LinearArgs p) {
       __syncthreads();
     }
     // the padding's ranks meet zeros of B, so they have to be finite
-    if ((groups & 1) && wv == NW - 1 && mine == ad) put(groups * 16 + 4 * q, floatx4{0.f, 0.f, 0.f, 0.f});
+    if ((groups & 1) && blockIdx.z == 0 && wv == NW - 1 && mine == ad) put(groups * 16 + 4 * q, floatx4{0.f, 0.f, 0.f, 0.f});
   }
 }
 
@@ -692,6 +699,7 @@ __device__ __forceinline__ void gemm_tile(const LinearArgs& p, uint8_t* smem, in
   constexpr int BB = KIND == kBI ? 1024 : 2048;  // weight bytes of a column group per step
   constexpr int SA = BM * 128, SB = BN / 16 * BB, SS = SA + SB;
   constexpr int AJ = BM / 8 / NW, BJ = SB / 1024 / NW, PER = AJ + BJ;
+  constexpr int LJ = BN / 16 / NW, LPER = AJ + LJ;  // of an adapters' step; LJ <= BJ
   static_assert(BM % (8 * NW) == 0 && SB % (1024 * NW) == 0 && BN / 16 % NW == 0, "whole loads per wave");
   constexpr int kOrder = KIND == kII ? 0 : 1;
   int (*const seg)[LORA ? BM : 1] = reinterpret_cast<int(*)[LORA ? BM : 1]>(segs);
@@ -752,9 +760,8 @@ __device__ __forceinline__ void gemm_tile(const LinearArgs& p, uint8_t* smem, in
   };
   const char* const ubase = reinterpret_cast<const char*>(p.u) + (size_t)r0 * rb * 128;
   auto issue_lora = [&](const Cursor& k, int s) {
-    constexpr int LB = BN / 16 / NW;
 #pragma unroll
-    for (int j = 0; j < LB; ++j) {
+    for (int j = 0; j < LJ; ++j) {
       const int cg = min(cg0 + wv + NW * j, p.cgs - 1);
       dma16(lane * 16, p.b + (((size_t)k.ad * p.cgs + cg) * rb + k.s) * 1024, stage_at(s, SA + (wv + NW * j) * 1024));
     }
@@ -765,8 +772,23 @@ __device__ __forceinline__ void gemm_tile(const LinearArgs& p, uint8_t* smem, in
             ubase + k.s * 128, stage_at(s, (wv + NW * j) * 1024));
     }
   };
+  // the adapters' steps take the ring's stages after the base steps
   Cursor next{rows, -1, rows, 0}, cur{rows, -1, rows, 0};
-  int issued = 0;  // adapters' steps; the k-th takes the ring's stage as base step steps + k would
+  const int steps = KIND == kII ? (p.kc + 1) >> 1 : p.kc;
+  int issued = steps;  // the first step whose loads are not under way (while base steps are left: that of the adapters')
+  auto issue_next = [&] {
+    if (next.at >= rows) return;
+    issue_lora(next, issued++);
+    advance(next);
+  };
+  // step s has landed, every wave is done with the stages before it, and of the steps behind
+  // it the last NS - 2 may be under way, if there are as many
+  auto lora_barrier = [&](int s) {
+    if (NS > 2 && issued - s > NS - 2)
+      vm_barrier<(NS - 2) * LPER>();
+    else
+      vm_barrier<0>();
+  };
   if constexpr (LORA) {
     enter(next, 0);
     cur = next;
@@ -820,10 +842,13 @@ __device__ __forceinline__ void gemm_tile(const LinearArgs& p, uint8_t* smem, in
     __builtin_amdgcn_sched_group_barrier(0x8, M, 0);
     __builtin_amdgcn_sched_barrier(0);
   };
-  const int steps = KIND == kII ? (p.kc + 1) >> 1 : p.kc;
 #pragma unroll
-  for (int s = 0; s < NS; ++s)
-    if (s < steps) issue(s);
+  for (int s = 0; s < NS; ++s) {
+    if (s < steps)
+      issue(s);
+    else if constexpr (LORA)
+      issue_next();
+  }
   if (steps >= NS)
     vm_barrier<(NS - 1) * PER>();
   else
@@ -850,13 +875,11 @@ __device__ __forceinline__ void gemm_tile(const LinearArgs& p, uint8_t* smem, in
     multiply(f0);
     interleave();
     if constexpr (decltype(tail)::value) {
-      vm_barrier<0>();
       if constexpr (LORA) {
-        // the adapters' first steps, while the last base steps run
-        if (next.at < rows) {
-          issue_lora(next, steps + issued++);
-          advance(next);
-        }
+        lora_barrier(s + 1);
+        issue_next();  // the adapters' first steps, while the last base steps run
+      } else {
+        vm_barrier<0>();
       }
     } else {
       vm_barrier<(NS - 2) * PER>();
@@ -899,11 +922,8 @@ __device__ __forceinline__ void gemm_tile(const LinearArgs& p, uint8_t* smem, in
   if constexpr (LORA) {
     const int w0 = wm * MI * 16;  // the wave's rows in the tile
     for (; cur.at < rows; advance(cur), ++s) {
-      vm_barrier<0>();  // step s has landed, and every wave is done with the one before
-      if (next.at < rows && issued - (s - steps) < NS) {
-        issue_lora(next, steps + issued++);
-        advance(next);
-      }
+      lora_barrier(s);
+      if (s > steps) issue_next();  // (the last base step's stage has its loads)
       const uint16_t* As = reinterpret_cast<const uint16_t*>(smem + (s % NS) * SS) + w0 * 64;
       const uint8_t* Bs = smem + (s % NS) * SS + SA + wn * NI * 1024 + c * 16;
       bf16x8 wf[2][NI];
@@ -918,17 +938,12 @@ __device__ __forceinline__ void gemm_tile(const LinearArgs& p, uint8_t* smem, in
         if (g0 + 16 <= cur.at || g0 >= cur.end) continue;
         const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(As + a_at<1>(m * 16 + c, 2 * q));
         const bf16x8 a1 = *reinterpret_cast<const bf16x8*>(As + a_at<1>(m * 16 + c, 2 * q + 1));
-        if (g0 >= cur.at && g0 + 16 <= cur.end) {
+        const bool mine = g0 + c >= cur.at && g0 + c < cur.end;
 #pragma unroll
-          for (int n = 0; n < NI; ++n) acc[m][n] = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, acc[m][n]));
-        } else {
-          const bool mine = g0 + c >= cur.at && g0 + c < cur.end;
+        for (int n = 0; n < NI; ++n) {
+          const floatx4 t = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, floatx4{0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
-          for (int n = 0; n < NI; ++n) {
-            const floatx4 t = mfma16(wf[1][n], a1, mfma16(wf[0][n], a0, floatx4{0.f, 0.f, 0.f, 0.f}));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[m][n][j] = mine ? acc[m][n][j] + t[j] : acc[m][n][j];
-          }
+          for (int j = 0; j < 4; ++j) acc[m][n][j] = mine ? acc[m][n][j] + t[j] : acc[m][n][j];
         }
       }
     }
@@ -1102,7 +1117,7 @@ void gemm(const LinearArgs& p, hipStream_t st) {
       gemm_of<KIND, 1, 4, 4, 2, 3>(p, st);
     else
       gemm_of<KIND, 2, 2, 2, 4, 2>(p, st);
-  } else if (mid > 32) {
+  } else if (mid > (p.adapter ? 96 : 32)) {
     if constexpr (KIND == kBI)
       gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
     else
@@ -1113,20 +1128,24 @@ void gemm(const LinearArgs& p, hipStream_t st) {
 }
 
 template <int KIND>
-void shrink(const LinearArgs& p, hipStream_t st) {
-  const dim3 grid((p.T + 15) / 16);
-  if (p.rank <= 16)
+void shrink(const LinearArgs& p, int adapters, hipStream_t st) {
+  // two blocks fill a CU: what the tiles leave of 256 goes to the groups, then to the adapters
+  const int tiles = (p.T + 15) / 16, groups = (p.rank + 15) / 16, room = std::max(256 / tiles, 1);
+  const int ng = groups <= room ? 1 : (groups <= 2 ? 2 : 4);
+  const int z = std::min((groups + ng - 1) / ng, room), y = std::min({room / z, 16, adapters});
+  const dim3 grid(tiles, y, z);
+  if (ng == 1)
     hipLaunchKernelGGL((k_lora_shrink<KIND, 1>), grid, dim3(1024), 0, st, p);
-  else if (p.rank <= 32)
+  else if (ng == 2)
     hipLaunchKernelGGL((k_lora_shrink<KIND, 2>), grid, dim3(1024), 0, st, p);
   else
     hipLaunchKernelGGL((k_lora_shrink<KIND, 4>), grid, dim3(1024), 0, st, p);
 }
 
 template <int KIND>
-void linear_kind(const LinearArgs& p, bool split, hipStream_t st) {
+void linear_kind(const LinearArgs& p, bool split, int adapters, hipStream_t st) {
   if (p.T <= kLinearDecodeTokens) return decode<KIND>(p, split, st);
-  if (p.adapter) shrink<KIND>(p, st);
+  if (p.adapter) shrink<KIND>(p, adapters, st);
   gemm<KIND>(p, st);
 }
 
@@ -1213,12 +1232,13 @@ hipError_t launch_linear(const kmoe_linear_weight& w, int64_t tokens, const void
   }
   p.part = reinterpret_cast<floatx4*>(ws + space.part);
   const bool split = linear_splits(w, tokens, x_dtype);
+  const int adapters = lora ? (int)lora->num_adapters : 0;
   if (x_dtype == KMOE_DTYPE_I8)
-    linear_kind<kII>(p, split, st);
+    linear_kind<kII>(p, split, adapters, st);
   else if (w.dtype == KMOE_DTYPE_I8)
-    linear_kind<kBI>(p, split, st);
+    linear_kind<kBI>(p, split, adapters, st);
   else
-    linear_kind<kBB>(p, split, st);
+    linear_kind<kBB>(p, split, adapters, st);
   return hipGetLastError();
 }
 
