@@ -16,7 +16,7 @@ constexpr int kLoraRankPad = 32;       // ranks of one step of the expanding pro
 constexpr int kLoraMaxRank = 256;
 constexpr int kLoraMaxAdapters = 1024;
 constexpr int kLoraSortBlock = 512;    // tokens per block of the sort
-constexpr int kLinearDecodeTokens = 64;  // above: the GEMM
+constexpr int kLinearDecodeTokens = 64;  // above: always tiles
 constexpr int kSplitSteps = 8;         // 128-byte steps of the rows that a block of the two-launch form takes
 
 }  // namespace kmoe
@@ -34,9 +34,11 @@ inline int64_t step_of(kmoe_dtype x) { return enum_value(x) == KMOE_DTYPE_I8 ? 1
 // Other rows are copied into the workspace first, padded with zeros.
 bool linear_rows_fit(const kmoe_linear_weight& w, const void* x, kmoe_dtype x_dtype, int64_t x_stride);
 
-// Whether a call of up to 64 tokens without adapters takes the two-launch form: the rows'
-// padded bytes exceed what every block of the single launch reads well (linear.hip).
-bool linear_splits(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype);
+// Which kernels a call runs (linear.hip): one launch in which every block reads all rows and
+// its columns' weights, two launches (partial sums, then their sum and the adapters'
+// part), or tiles of rows and columns.
+enum class LinearForm { kOne, kSplit, kTiles };
+LinearForm linear_form(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, bool lora);
 
 // Byte offsets of the workspace: the copied rows (0, where they are copied), partial sums
 // (two-launch form), the adapters' inner values.

@@ -299,7 +299,8 @@ __device__ __forceinline__ void shrink_row(const LinearArgs& p, int t, int g, fl
 // pass per adapter of the tile and NG groups of 16 ranks; u as bf16 hi + lo. The passes are
 // shared out over the blocks of the tile (y: the adapters, z: the groups). Bound by
 // latency: the tile's adapters come with its rows, and all chunks of 4096 elements are in
-// flight together.
+// flight together. 128 rows of 64 adapters and rank 64, 2048 inputs: 32.5 us with one block
+// per tile, about 8 with the passes shared out.
 // ---------------------------------------------------------------------------
 template <int KIND, int NG>
 __global__ __launch_bounds__(1024) void k_lora_shrink(LinearArgs p) {
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(1024) void k_lora_shrink(LinearArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens without adapters: the weights stream through registers once. A block takes 16 CG
+// Few tokens without adapters (LinearForm::kOne): the weights stream through registers once. A block takes 16 CG
 // columns for all rows, its eight waves an eighth of the chunks each; the partial sums meet
 // in LDS in wave order. Bound by latency: a wave requests NB chunks at once (the whole of its
 // share up to 2048 inputs).
@@ -509,7 +510,7 @@ __global__ __launch_bounds__(512) void k_linear_decode(LinearArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens in two launches. The first: blocks of 128 columns and eight steps (128 bytes of
+// Few tokens in two launches (LinearForm::kSplit). The first: blocks of 128 columns and eight steps (128 bytes of
 // each row), every load of a block in flight at once - the rows through LDS, shared by NW
 // waves of 16 CG columns, the weights in registers - whose partial sums go to the workspace;
 // and beside them the blocks of the adapters' u, which thus costs no launch of its own. The
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(64) void k_linear_finish(LinearArgs p, int splits) 
 }
 
 // ---------------------------------------------------------------------------
-// Above 64 tokens: a GEMM over tiles of BM rows and BN columns. Steps of 128 bytes of
+// Many tokens or columns (LinearForm::kTiles): a GEMM over tiles of BM rows and BN columns. Steps of 128 bytes of
 // every row (64 bf16, 128 int8) and the columns' weights of the same depth reach LDS by direct
 // loads, a ring of NS stages. Rows as [row][8 x 16 B] with the pieces swizzled by row
 // (a_piece_at), the weights in the packed order, which is the order their lanes read. The
@@ -678,10 +679,11 @@ __global__ __launch_bounds__(64) void k_linear_finish(LinearArgs p, int splits) 
 //
 // With adapters the rows are the sorted ones, so a tile meets few adapters. After the
 // base sum, scaled to f32, each adapter of the tile adds steps of 32 ranks in the same
-// ring: the tile's rows of u (hi and lo, 128 bytes) times the adapter's B. A 16-row group
-// that lies wholly in the adapter's range adds in place; one that does not computes the
-// product apart and takes its own rows by selection, so that nothing of another adapter (an
-// infinity times zero) reaches a row.
+// ring: the tile's rows of u (hi and lo, 128 bytes) times the adapter's B. The product of a
+// 16-row group is computed apart and added to the adapter's own rows by selection, so that
+// nothing of another adapter (an infinity times zero) reaches a row, and a row's sums are the
+// same whatever its neighbours take (adding in place where a group is of one adapter was no
+// faster).
 // ---------------------------------------------------------------------------
 template <int KIND, int WM, int WN, int MI, int NI, int NS, bool LORA>
 struct GemmShape {
@@ -1031,11 +1033,7 @@ dim3 grid_for(int64_t items) {
 
 template <int KIND, int RB>
 void decode_of(const LinearArgs& p, bool split, hipStream_t st) {
-  // Adapters, or rows of more than 256 KB, which every block of the single launch reads whole:
-  // two launches. bf16 rows, int8 weights, us (single, two launches): 64 x 4096 -> 2048 18.4,
-  // 10.9; 64 x 8192 -> 4096 33.8, 23.6; but 64 x 2048 -> 5120 11.5, 12.4; 24 x 2048 -> 5120
-  // 6.6, 9.1; one row 2048 -> 5120 4.4, 6.8.
-  if (p.adapter || split) {
+  if (split) {
     // eight waves of 16 columns share the rows' LDS reads less than four of 32, but convert
     // and load beside more others: 24 rows of rank 64, 4096 -> 9216, 23.0 us on bf16 rows
     // (four 28.9), on int8 rows, which take half the LDS and no conversion, 22.6 (four 19.5)
@@ -1045,11 +1043,12 @@ void decode_of(const LinearArgs& p, bool split, hipStream_t st) {
     hipLaunchKernelGGL((k_linear_split<KIND, RB, NW, CG>), dim3(shrink + blocks), dim3(64 * NW), 0, st, p, splits,
                        shrink);
     hipLaunchKernelGGL((k_linear_finish<KIND>), dim3((p.cgs * 4 + 63) / 64, p.T), dim3(64), 0, st, p, splits);
-  } else if (p.cgs <= 256) {
+  } else if (RB == 4 || p.cgs <= 256) {
     // one column group per block while that is no more than a block per CU (one row 8192 ->
-    // 4096 7.7 us, two groups 10.8); above, two, which share the rows (24 x 2048 -> 5120 6.6, one 8.9)
+    // 4096 7.7 us, two groups 10.8); above, which four row groups never are here (linear_form),
+    // two, which share the rows (24 x 2048 -> 5120 6.6, one 8.9)
     hipLaunchKernelGGL((k_linear_decode<KIND, RB, 1>), dim3(p.cgs), dim3(512), 0, st, p);
-  } else {
+  } else if constexpr (RB < 4) {
     hipLaunchKernelGGL((k_linear_decode<KIND, RB, 2>), dim3((p.cgs + 1) / 2), dim3(512), 0, st, p);
   }
 }
@@ -1092,6 +1091,10 @@ void gemm_of(const LinearArgs& p, hipStream_t st) {
 //   2048 -> 5120, 2048 (640; m = 160) bf16 x int8 74.6  55.5  47.9  48.6  55.3
 //   2560 -> 6144, 2048 (768; m = 192)       bf16 119.7  93.6  74.2  70.1  64.2
 //   4096 -> 9216, 2048 (1152; m = 288)      int8 153.3 111.7  90.2  87.6  75.6 (quarters in the last round)
+// A tile is not much taller than the rows: 64 rows 2048 -> 151936 in tiles of 256 rows 152 us,
+// of 64 114; 300 x 4096 -> 9216 in tiles of 256 46.9, of 128 37.7; but 160 x 2048 -> 151936 166, 182.
+// With adapters, of which a low tile meets fewer, 32 x 64 up to 96 tiles of 128 x 128: 128 rows
+// of as many requests, 64 adapters of rank 64, 2048 -> 5120 37.0 in tiles of 64, 29.2 of 32.
 // The smaller tiles are bound by LDS reads, so their four waves stand 2 x 2; int8 weights with
 // bf16 rows, which each wave converts for itself, want them 1 x 4 (64 x 64: 2048 -> 5120, 512
 // rows 19.0 against 21.3, bf16 weights 22.8 against 22.0).
@@ -1099,7 +1102,7 @@ template <int KIND>
 void gemm(const LinearArgs& p, hipStream_t st) {
   const int tm = (p.T + 255) / 256, tn = (p.cgs + 15) / 16;
   const int64_t big = (int64_t)tm * tn, mid = (int64_t)((p.T + 127) / 128) * ((p.cgs + 7) / 8);
-  if (big >= 176) {
+  if (big >= 176 && (int64_t)tm * 256 * 3 <= (int64_t)p.T * 5) {
     // what is left after the whole rounds goes in quarters, unless those would take four rounds
     const int64_t rest = big % 256;
     const bool quarters = big > 256 && rest <= 192;
@@ -1110,14 +1113,14 @@ void gemm(const LinearArgs& p, hipStream_t st) {
     else
       hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, false>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn,
                          (int)whole);
-  } else if (mid >= 400) {
+  } else if (mid >= 400 && p.T > 64) {
     gemm_of<KIND, 2, 2, 4, 4, 2>(p, st);
-  } else if (mid >= (KIND == kBI ? 224 : 144)) {
+  } else if (mid >= (KIND == kBI ? 224 : 144) && p.T > 32) {
     if constexpr (KIND == kBI)
       gemm_of<KIND, 1, 4, 4, 2, 3>(p, st);
     else
       gemm_of<KIND, 2, 2, 2, 4, 2>(p, st);
-  } else if (mid > (p.adapter ? 96 : 32)) {
+  } else if (mid > (p.adapter ? 96 : 32) && p.T > 32) {
     if constexpr (KIND == kBI)
       gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
     else
@@ -1129,7 +1132,8 @@ void gemm(const LinearArgs& p, hipStream_t st) {
 
 template <int KIND>
 void shrink(const LinearArgs& p, int adapters, hipStream_t st) {
-  // two blocks fill a CU: what the tiles leave of 256 goes to the groups, then to the adapters
+  // one block per CU: what the tiles leave of them goes to the groups, then to the adapters (up to
+  // two per CU was no faster for 128 rows and cost 4096 rows 2 us)
   const int tiles = (p.T + 15) / 16, groups = (p.rank + 15) / 16, room = std::max(256 / tiles, 1);
   const int ng = groups <= room ? 1 : (groups <= 2 ? 2 : 4);
   const int z = std::min((groups + ng - 1) / ng, room), y = std::min({room / z, 16, adapters});
@@ -1143,8 +1147,8 @@ void shrink(const LinearArgs& p, int adapters, hipStream_t st) {
 }
 
 template <int KIND>
-void linear_kind(const LinearArgs& p, bool split, int adapters, hipStream_t st) {
-  if (p.T <= kLinearDecodeTokens) return decode<KIND>(p, split, st);
+void linear_kind(const LinearArgs& p, LinearForm form, int adapters, hipStream_t st) {
+  if (form != LinearForm::kTiles) return decode<KIND>(p, form == LinearForm::kSplit, st);
   if (p.adapter) shrink<KIND>(p, adapters, st);
   gemm<KIND>(p, st);
 }
@@ -1231,14 +1235,14 @@ hipError_t launch_linear(const kmoe_linear_weight& w, int64_t tokens, const void
     p.u = ws + space.u;
   }
   p.part = reinterpret_cast<floatx4*>(ws + space.part);
-  const bool split = linear_splits(w, tokens, x_dtype);
+  const LinearForm form = linear_form(w, tokens, x_dtype, lora != nullptr);
   const int adapters = lora ? (int)lora->num_adapters : 0;
   if (x_dtype == KMOE_DTYPE_I8)
-    linear_kind<kII>(p, split, adapters, st);
+    linear_kind<kII>(p, form, adapters, st);
   else if (w.dtype == KMOE_DTYPE_I8)
-    linear_kind<kBI>(p, split, adapters, st);
+    linear_kind<kBI>(p, form, adapters, st);
   else
-    linear_kind<kBB>(p, split, adapters, st);
+    linear_kind<kBB>(p, form, adapters, st);
   return hipGetLastError();
 }
 

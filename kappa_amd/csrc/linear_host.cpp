@@ -43,15 +43,35 @@ bool linear_rows_fit(const kmoe_linear_weight& w, const void* x, kmoe_dtype x_dt
          x_stride * (int64_t)dtype_size(x_dtype) % 16 == 0;
 }
 
-bool linear_splits(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype) {
-  const int64_t chunks = (w.in_features + 63) / 64 * 64 * (int64_t)dtype_size(x_dtype);
-  return tokens > 0 && tokens <= kmoe::kLinearDecodeTokens && round_up(tokens, 16) * chunks > 256 * 1024;
+LinearForm linear_form(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, bool lora) {
+  if (tokens > kmoe::kLinearDecodeTokens) return LinearForm::kTiles;
+  if (lora) return LinearForm::kSplit;
+  // Above 16 rows the one launch grows with the 16-row groups times the column groups, the tiles
+  // do not. us (one or two launches, tiles), bf16 / bf16 x int8 / int8:
+  //   17 x 4096 -> 9216   (1152)   23.7, 14.0 /  18.0, 15.2 /  12.7, 9.2
+  //   32 x 2048 -> 6144    (768)    9.1,  9.6 /   7.6, 10.1 /   6.3, 7.1
+  //   48 x 2048 -> 5120    (960)   10.6,  9.7 /   9.4, 10.2 /   7.2, 7.1
+  //   64 x 2048 -> 5120   (1280)   12.8,  9.8 /  11.5, 10.6 /   8.3, 7.2
+  //   64 x 4096 -> 2048    (512)   12.3, 14.0 /  10.8, 15.2 /  12.0, 8.6
+  //   64 x 2048 -> 151936 (37984)  210,   114 /   188, 68   /   134, 65
+  // Up to 16 rows: 16 x 2048 -> 16384 13.5, 12.3 / 9.7, 9.6 / 8.7, 8.1; one row -> 151936 93,
+  // 102 / 51, 55 / 49, 53; but where the one launch's blocks (of two column groups) make a
+  // full round of 256 CUs and a small one, 4096 -> 9216, one row 18.6, 13.5 / 10.3, 14.6 / 9.2, 8.7.
+  const bool converts = enum_value(x_dtype) == KMOE_DTYPE_BF16 && enum_value(w.dtype) == KMOE_DTYPE_I8;
+  const int64_t rows = (tokens + 15) / 16, columns = padded_out(w.out_features) / 16;
+  if (rows > 1 ? rows * columns > (converts ? 1024 : 896) : !converts && columns > 512 && columns < 768)
+    return LinearForm::kTiles;
+  // Every block of the one launch reads all rows: two launches above 256 KB of them. us (one,
+  // two), bf16 rows and int8 weights: 64 x 4096 -> 2048 18.4, 10.9; 64 x 8192 -> 4096 33.8, 23.6;
+  // but 24 x 2048 -> 5120 6.6, 9.1; one row 2048 -> 5120 4.4, 6.8.
+  const int64_t row_bytes = (w.in_features + 63) / 64 * 64 * (int64_t)dtype_size(x_dtype);
+  return rows * 16 * row_bytes > 256 * 1024 ? LinearForm::kSplit : LinearForm::kOne;
 }
 
 LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora,
                          bool copied) {
   const size_t T = (size_t)tokens, in = (size_t)padded_in(w.in_features);
-  const bool splits = tokens <= kmoe::kLinearDecodeTokens && (lora || linear_splits(w, tokens, x_dtype));
+  const bool splits = linear_form(w, tokens, x_dtype, lora) == LinearForm::kSplit;
   const size_t parts = (in / (size_t)step_of(x_dtype) + kmoe::kSplitSteps - 1) / kmoe::kSplitSteps;
   LinearSpace s;
   s.part = copied ? align256(T * in * dtype_size(x_dtype)) : 0;
@@ -62,11 +82,13 @@ LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype
 }
 
 size_t linear_most_bytes(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora) {
-  const size_t own = linear_space(w, tokens, x_dtype, lora, true).total;
-  if (tokens <= kmoe::kLinearDecodeTokens) return own;
-  // just above the sizes that hold partial sums
-  const size_t below = linear_space(w, kmoe::kLinearDecodeTokens, x_dtype, lora, true).total;
-  return own > below ? own : below;
+  size_t most = linear_space(w, tokens, x_dtype, lora, true).total;
+  // fewer tokens may hold partial sums where these do not; the form changes with the 16-row groups
+  for (int64_t t = 16; t <= kmoe::kLinearDecodeTokens && t < tokens; t += 16) {
+    const size_t s = linear_space(w, t, x_dtype, lora, true).total;
+    if (s > most) most = s;
+  }
+  return most;
 }
 
 kmoe_status check_linear_weight(const kmoe_linear_weight* w, bool buffers) {

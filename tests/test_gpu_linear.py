@@ -108,7 +108,7 @@ def test_linear(dev, T, K, N, weights, rows):
 
 # every tile of the GEMM, with rows and columns that end inside one
 TILES = [(513, 192, 500), (1100, 128, 2100), (1900, 64, 2000), (2100, 128, 2001),
-         (2900, 64, 2400), (3000, 192, 3900), (4200, 128, 4001),
+         (2900, 64, 2400), (3, 64, 9000), (17, 128, 9000), (33, 192, 6000), (64, 100, 4500), (3000, 192, 3900), (4200, 128, 4001),
          (5400, 64, 5290)]  # fmt: skip
 
 
@@ -210,6 +210,25 @@ def test_what_is_not_finite_stays_in_its_rows(dev, T, bad):
     y = linear(x2, p, lora=prepack_lora(a, b, f), batch=lora_batch(ad, L))
     other = torch.arange(T, device=dev) != 3
     assert torch.equal(y[other], want[other]) and not torch.isfinite(y[3]).any()
+
+
+@pytest.mark.parametrize("T,K,N", [(8, 256, 96), (100, 256, 96), (300, 192, 1000), (700, 128, 2600), (2900, 64, 2400)])
+@pytest.mark.parametrize("R", [16, 70])
+def test_a_row_keeps_its_bits_whatever_its_neighbours_take(dev, T, K, N, R):
+    """The adapters of every third token stay, those of the others change (all of one, one
+    each, none): the sorted order, the tiles' ranges and the neighbours do, the row does not."""
+    from kappa_amd.qwen3 import linear, lora_batch, prepack_linear, prepack_lora
+
+    L = 40
+    x, w, _, _ = make(dev, T, K, N)
+    a, b, f, ad = make_adapters(dev, T, K, N, L, R)
+    p, l = prepack_linear(w), prepack_lora(a, b, f)
+    t = torch.arange(T, device=dev)
+    stay = t % 3 == 0
+    want = linear(x, p, lora=l, batch=lora_batch(ad, L))[stay]
+    for other in (torch.full_like(ad, 5), (t % L).to(ad.dtype), torch.full_like(ad, -1)):
+        y = linear(x, p, lora=l, batch=lora_batch(torch.where(stay, ad, other), L))
+        assert torch.equal(y[stay], want)
 
 
 @pytest.mark.parametrize("T", [6, 90])
