@@ -122,7 +122,7 @@ def add_rms_norm_q8(
             return add_rms_norm_q8(x, residual, sc, epsilon=epsilon)
     h = x if residual is None else torch.empty_like(x)
     q = torch.empty_like(x, dtype=torch.int8)
-    s = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=dev)
+    s = x.new_empty((*x.shape[:-1], 1), dtype=torch.float32)
     _lib.check(
         _lib.lib().kmoe_add_rms_norm_q8(
             desc, x.data_ptr(), None if residual is None else residual.data_ptr(), sc.data_ptr(), _CODE[sc.dtype],

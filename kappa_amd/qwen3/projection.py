@@ -280,8 +280,8 @@ def linear(
     L = _lib.lib()
     n = ctypes.c_size_t()
     _lib.check(L.kmoe_linear_call_bytes(w.struct, T, v.data_ptr(), code, stride, ls, ctypes.byref(n)))
-    out = torch.empty((*shape, w.out_features), dtype=torch.bfloat16, device=dev)
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
+    out = v.new_empty((*shape, w.out_features), dtype=torch.bfloat16)
+    ws = v.new_empty(n.value, dtype=torch.uint8) if n.value else None
     _lib.check(
         L.kmoe_linear(
             w.struct, T, v.data_ptr(), code, stride, xs, ls, bs, out.data_ptr(),
