@@ -1034,10 +1034,13 @@ dim3 grid_for(int64_t items) {
 template <int KIND, int RB>
 void decode_of(const LinearArgs& p, bool split, hipStream_t st) {
   if (split) {
-    // eight waves of 16 columns share the rows' LDS reads less than four of 32, but convert
-    // and load beside more others: 24 rows of rank 64, 4096 -> 9216, 23.0 us on bf16 rows
-    // (four 28.9), on int8 rows, which take half the LDS and no conversion, 22.6 (four 19.5)
-    constexpr int NW = KIND == kII ? 4 : 8, CG = KIND == kII ? 2 : 1, ST = kSplitSteps;
+    // Up to 32 rows bf16 rows take eight waves of 16 columns, int8 rows, which take half the LDS
+    // and no conversion, four of 32; above, where a block's rows fill more of the LDS, both
+    // take four of 16, so that more blocks run. us, 24 rows of rank 64, 4096 -> 9216: int8
+    // weights 23.1 (four of 16 28.9), int8 rows 19.6 (28.2); 64 rows of rank 16, 4096 -> 2048, bf16
+    // weights 16.3 with eight, 13.9 with four of 16, int8 rows 12.5 with four of 32, 11.0; 48 rows
+    // 15.3, 13.1 and 11.5, 10.3.
+    constexpr int NW = RB > 2 || KIND == kII ? 4 : 8, CG = RB < 3 && KIND == kII ? 2 : 1, ST = kSplitSteps;
     const int steps = KIND == kII ? (p.kc + 1) / 2 : p.kc, splits = (steps + ST - 1) / ST;
     const int blocks = (p.cgs + NW * CG - 1) / (NW * CG) * splits, shrink = p.adapter ? p.T * ((p.rank + 15) / 16) : 0;
     hipLaunchKernelGGL((k_linear_split<KIND, RB, NW, CG>), dim3(shrink + blocks), dim3(64 * NW), 0, st, p, splits,
