@@ -299,8 +299,8 @@ __device__ __forceinline__ void shrink_row(const LinearArgs& p, int t, int g, fl
 // pass per adapter of the tile and NG groups of 16 ranks; u as bf16 hi + lo. The passes are
 // shared out over the blocks of the tile (y: the adapters, z: the groups). Bound by
 // latency: the tile's adapters come with its rows, and all chunks of 4096 elements are in
-// flight together. 128 rows of 64 adapters and rank 64, 2048 inputs: 32.5 us with one block
-// per tile, about 8 with the passes shared out.
+// flight together. 128 rows of 64 adapters and rank 64, 2048 -> 5120: the call took 69.6 us with
+// one block per tile (32.5 of them here), 40.4 with the passes shared out.
 // ---------------------------------------------------------------------------
 template <int KIND, int NG>
 __global__ __launch_bounds__(1024) void k_lora_shrink(LinearArgs p) {

@@ -187,6 +187,24 @@ def test_sizes():
     assert L.kmoe_linear_call_bytes(lin(), 4, P, BF, -1, None, b) == _lib.ERR_INVALID_ARG
 
 
+def test_the_workspace_of_many_tokens_serves_fewer():
+    """The kernels change with the number of tokens, and so does what a call needs: partial sums
+    for some sizes up to 64 tokens, none for others."""
+    L = _lib.lib()
+    most, call = ctypes.c_size_t(), ctypes.c_size_t()
+    for K, N in ((8192, 4096), (8192, 3500), (65536, 64), (4096, 9216), (100, 20000)):
+        for l in (None, lora(R=40, K=K, N=N)):
+            for dtype, x_dtype in ((BF, BF), (I8, BF), (I8, I8)):
+                w = lin(K=K, N=N, dtype=dtype)
+                need = 0
+                for T in range(1, 100):
+                    for x in (P, P + 2):
+                        assert L.kmoe_linear_call_bytes(w, T, x, x_dtype, K, l, call) == _lib.OK
+                        need = max(need, call.value)
+                    assert L.kmoe_linear_workspace_bytes(w, T, x_dtype, l, most) == _lib.OK
+                    assert most.value >= need
+
+
 def test_python_layer_refuses_cpu_tensors():
     from kappa_amd.qwen3 import LoraAdapters, add_rms_norm, add_rms_norm_q8, lora_batch, prepack_linear, prepack_lora
 
