@@ -290,7 +290,7 @@ kmoe_status kmoe_add_rms_norm(const kmoe_desc* desc, const void* x, const void* 
 
 /* The same with the normalised rows in 8 bits: with v = (h * r) * scale in f32 (not rounded
  * to the activation dtype) and m the row's largest |v|,
- *   q_scale[t] = max(m / 127, FLT_MIN),  q = clip(rint(v * (1 / q_scale)), -127, 127).
+ *   q_scale[t] = max(m / 127, FLT_MIN),  q = clip(rint(v / q_scale), -127, 127).
  * A row that holds an infinity or a NaN has q_scale = NaN and q = 0, so whatever is
  * computed from it is NaN. residual and h_out may both be NULL: h = x. */
 kmoe_status kmoe_add_rms_norm_q8(const kmoe_desc* desc, const void* x, const void* residual, const void* scale,

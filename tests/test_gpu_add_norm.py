@@ -106,6 +106,27 @@ def test_q8_against_the_formula(dev, T, D, act):
     assert h2 is h and torch.equal(q2.values, q.values) and torch.equal(q2.scale, q.scale)
 
 
+@pytest.mark.parametrize("T,D,act", [(2048, 4096, "bf16"), (1024, 4096, "f32"), (17000, 500, "bf16"), (9, 4095, "bf16")])
+def test_q8_is_the_rounded_quotient(dev, T, D, act):
+    """Bit for bit rint(v / s): v in f32 is what rms_norm gives for the same rows in float32,
+    the division rounds once (done here on the CPU)."""
+    from kappa_amd.qwen3 import add_rms_norm_q8, rms_norm
+
+    x, res, scale = _case(dev, T, D, act, "bf16", 8)
+    if act == "f32":  # every fourth row so small that its scale is near, or at, the smallest float
+        x[::4] *= 2.0**-113
+        res[::4] *= 2.0**-113
+        x[::8] *= 2.0**-8
+        res[::8] *= 2.0**-8
+    q, h = add_rms_norm_q8(x, res, scale, epsilon=EPS)
+    v = rms_norm(h.float(), scale.float(), epsilon=EPS).cpu()
+    s = torch.clamp_min(v.abs().amax(dim=1, keepdim=True) / 127.0, TINY)
+    assert torch.equal(q.scale.cpu(), s)
+    want = torch.clamp(torch.round(v / s), -127.0, 127.0)
+    got = q.values.cpu().float()
+    assert torch.equal(got, want), int((got != want).sum())
+
+
 @pytest.mark.parametrize("D", [128, 100, 4096])
 def test_q8_rows_at_the_edges(dev, D):
     """Zero rows, tiny rows, and rows with an infinity or a NaN, beside an ordinary one."""
