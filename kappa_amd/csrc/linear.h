@@ -40,6 +40,28 @@ bool linear_rows_fit(const kmoe_linear_weight& w, const void* x, kmoe_dtype x_dt
 enum class LinearForm { kOne, kSplit, kTiles };
 LinearForm linear_form(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, bool lora);
 
+// Column groups (16 columns) that a block of the one launch takes; cgs: groups of the packed weights
+int decode_groups(int64_t cgs);
+
+// The tiles' size, rows x columns; converts: bf16 rows with int8 weights
+enum class LinearTile { k32x64, k64x64, k64x128, k128x128, k256x256 };
+LinearTile linear_tile(int64_t tokens, int64_t cgs, bool converts, bool lora);
+
+// The blocks of the 256 x 256 tiles: the first `whole` take one each (a multiple of 8, those past
+// the last nothing), the others a quarter
+struct LinearRounds {
+  int64_t whole, blocks;
+};
+LinearRounds linear_rounds(int64_t tiles);
+
+// The adapters' inner products above 64 tokens, per 16 rows: groups of 16 ranks that a block
+// sums at a time (1, 2 or 4), and how many blocks share the adapters (y) and the groups (z)
+struct LoraShrink {
+  int groups;
+  unsigned y, z;
+};
+LoraShrink lora_shrink(int64_t tokens, int64_t rank, int64_t adapters);
+
 // Byte offsets of the workspace: the copied rows (0, where they are copied), partial sums
 // (two-launch form), the adapters' inner values.
 struct LinearSpace {

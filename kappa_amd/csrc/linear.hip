@@ -9,7 +9,6 @@
 // Three kinds of products (Kind): bf16 rows with bf16 or int8 weights on
 // v_mfma_f32_16x16x32_bf16 (int8 becomes bf16 in registers, exactly), and int8 rows
 // with int8 weights on v_mfma_i32_16x16x64_i8, whose sums are exact.
-#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -1046,10 +1045,7 @@ void decode_of(const LinearArgs& p, bool split, hipStream_t st) {
     hipLaunchKernelGGL((k_linear_split<KIND, RB, NW, CG>), dim3(shrink + blocks), dim3(64 * NW), 0, st, p, splits,
                        shrink);
     hipLaunchKernelGGL((k_linear_finish<KIND>), dim3((p.cgs * 4 + 63) / 64, p.T), dim3(64), 0, st, p, splits);
-  } else if (RB == 4 || p.cgs <= 256) {
-    // one column group per block while that is no more than a block per CU (one row 8192 ->
-    // 4096 7.7 us, two groups 10.8); above, which four row groups never are here (linear_form),
-    // two, which share the rows (24 x 2048 -> 5120 6.6, one 8.9)
+  } else if (RB == 4 || decode_groups(p.cgs) == 1) {  // (four row groups never take two: linear_form)
     hipLaunchKernelGGL((k_linear_decode<KIND, RB, 1>), dim3(p.cgs), dim3(512), 0, st, p);
   } else if constexpr (RB < 4) {
     hipLaunchKernelGGL((k_linear_decode<KIND, RB, 2>), dim3((p.cgs + 1) / 2), dim3(512), 0, st, p);
@@ -1081,69 +1077,47 @@ void gemm_of(const LinearArgs& p, hipStream_t st) {
     hipLaunchKernelGGL((k_linear_gemm<KIND, WM, WN, MI, NI, NS, false>), grid, dim3(64 * WM * WN), 0, st, p, tm, tn);
 }
 
-// The tile by how many there are, against 256 CUs. Times in us of tiles of 32 x 64, 64 x 64,
-// 64 x 128, 128 x 128 and 256 x 256, for n tiles of 128 x 128 (m of 256 x 256):
-//   1024 -> 512, 1024 rows (n = 32)  bf16 x int8   6.2   7.4   9.9  13.8  28.4
-//   4096 -> 2048, 333 (48)           bf16 x int8  19.6  18.6  26.8  39.3  83.6
-//   2560 -> 6144, 200 / 512 (96, 192)       bf16  19.7 / 35.5, 16.4 / 26.6, 23.0 / 25.3, 27.5 / 28.0
-//   4096 -> 2048, 1500 (192)         bf16 x int8  46.6  34.5  37.2  39.9  84.3
-//   2048 -> 5120, 700 (240)          bf16 x int8  28.8  25.2  22.5  24.6  48.8
-//   4096 -> 9216, 333 / 512 (216, 288)      int8  32.7 / 42.6, 26.2 / 33.3, 22.0 / 29.3, 25.3 / 33.3
-//   2560 -> 6144, 1024 (384)                bf16  62.3  48.6  39.4  40.3  59.3
-//   2048 -> 5120, 1500 (480)                bf16  63.7  47.9  43.0  34.7  51.2
-//   2048 -> 5120, 2048 (640; m = 160) bf16 x int8 74.6  55.5  47.9  48.6  55.3
-//   2560 -> 6144, 2048 (768; m = 192)       bf16 119.7  93.6  74.2  70.1  64.2
-//   4096 -> 9216, 2048 (1152; m = 288)      int8 153.3 111.7  90.2  87.6  75.6 (quarters in the last round)
-// A tile is not much taller than the rows: 64 rows 2048 -> 151936 in tiles of 256 rows 152 us,
-// of 64 114; 300 x 4096 -> 9216 in tiles of 256 46.9, of 128 37.7; but 160 x 2048 -> 151936 166, 182.
-// With adapters, of which a low tile meets fewer, 32 x 64 up to 96 tiles of 128 x 128: 128 rows
-// of as many requests, 64 adapters of rank 64, 2048 -> 5120 37.0 in tiles of 64, 29.2 of 32.
-// The smaller tiles are bound by LDS reads, so their four waves stand 2 x 2; int8 weights with
-// bf16 rows, which each wave converts for itself, want them 1 x 4 (64 x 64: 2048 -> 5120, 512
-// rows 19.0 against 21.3, bf16 weights 22.8 against 22.0).
 template <int KIND>
 void gemm(const LinearArgs& p, hipStream_t st) {
-  const int tm = (p.T + 255) / 256, tn = (p.cgs + 15) / 16;
-  const int64_t big = (int64_t)tm * tn, mid = (int64_t)((p.T + 127) / 128) * ((p.cgs + 7) / 8);
-  if (big >= 176 && (int64_t)tm * 256 * 3 <= (int64_t)p.T * 5) {
-    // what is left after the whole rounds goes in quarters, unless those would take four rounds
-    const int64_t rest = big % 256;
-    const bool quarters = big > 256 && rest <= 192;
-    const int64_t whole = quarters ? big - rest : (big + 7) / 8 * 8, blocks = whole + (quarters ? (4 * rest + 7) / 8 * 8 : 0);
-    if (p.adapter)
-      hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, true>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn,
-                         (int)whole);
-    else
-      hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, false>), dim3((unsigned)blocks), dim3(512), 0, st, p, tm, tn,
-                         (int)whole);
-  } else if (mid >= 400 && p.T > 64) {
-    gemm_of<KIND, 2, 2, 4, 4, 2>(p, st);
-  } else if (mid >= (KIND == kBI ? 224 : 144) && p.T > 32) {
-    if constexpr (KIND == kBI)
-      gemm_of<KIND, 1, 4, 4, 2, 3>(p, st);
-    else
-      gemm_of<KIND, 2, 2, 2, 4, 2>(p, st);
-  } else if (mid > (p.adapter ? 96 : 32) && p.T > 32) {
-    if constexpr (KIND == kBI)
-      gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
-    else
-      gemm_of<KIND, 2, 2, 2, 2, 4>(p, st);
-  } else {
-    gemm_of<KIND, 1, 4, 2, 1, 4>(p, st);
+  // The smaller tiles are bound by LDS reads, so their four waves stand 2 x 2; int8 weights with
+  // bf16 rows, which each wave converts for itself, want them 1 x 4 (64 x 64: 2048 -> 5120, 512
+  // rows 19.0 against 21.3, bf16 weights 22.8 against 22.0).
+  switch (linear_tile(p.T, p.cgs, KIND == kBI, p.adapter != nullptr)) {
+    case LinearTile::k256x256: {
+      const int tm = (p.T + 255) / 256, tn = (p.cgs + 15) / 16;
+      const LinearRounds r = linear_rounds((int64_t)tm * tn);
+      if (p.adapter)
+        hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, true>), dim3((unsigned)r.blocks), dim3(512), 0, st, p, tm, tn,
+                           (int)r.whole);
+      else
+        hipLaunchKernelGGL((k_linear_gemm_mixed<KIND, false>), dim3((unsigned)r.blocks), dim3(512), 0, st, p, tm, tn,
+                           (int)r.whole);
+      return;
+    }
+    case LinearTile::k128x128:
+      return gemm_of<KIND, 2, 2, 4, 4, 2>(p, st);
+    case LinearTile::k64x128:
+      if constexpr (KIND == kBI)
+        return gemm_of<KIND, 1, 4, 4, 2, 3>(p, st);
+      else
+        return gemm_of<KIND, 2, 2, 2, 4, 2>(p, st);
+    case LinearTile::k64x64:
+      if constexpr (KIND == kBI)
+        return gemm_of<KIND, 1, 4, 4, 1, 4>(p, st);
+      else
+        return gemm_of<KIND, 2, 2, 2, 2, 4>(p, st);
+    case LinearTile::k32x64:
+      return gemm_of<KIND, 1, 4, 2, 1, 4>(p, st);
   }
 }
 
 template <int KIND>
 void shrink(const LinearArgs& p, int adapters, hipStream_t st) {
-  // one block per CU: what the tiles leave of them goes to the groups, then to the adapters (up to
-  // two per CU was no faster for 128 rows and cost 4096 rows 2 us)
-  const int tiles = (p.T + 15) / 16, groups = (p.rank + 15) / 16, room = std::max(256 / tiles, 1);
-  const int ng = groups <= room ? 1 : (groups <= 2 ? 2 : 4);
-  const int z = std::min((groups + ng - 1) / ng, room), y = std::min({room / z, 16, adapters});
-  const dim3 grid(tiles, y, z);
-  if (ng == 1)
+  const LoraShrink s = lora_shrink(p.T, p.rank, adapters);
+  const dim3 grid((p.T + 15) / 16, s.y, s.z);
+  if (s.groups == 1)
     hipLaunchKernelGGL((k_lora_shrink<KIND, 1>), grid, dim3(1024), 0, st, p);
-  else if (ng == 2)
+  else if (s.groups == 2)
     hipLaunchKernelGGL((k_lora_shrink<KIND, 2>), grid, dim3(1024), 0, st, p);
   else
     hipLaunchKernelGGL((k_lora_shrink<KIND, 4>), grid, dim3(1024), 0, st, p);

@@ -2,6 +2,8 @@
 // is made here; the entry points in linear_api.hip run these checks first.
 #include "linear.h"
 
+#include <algorithm>
+
 namespace kmoe_host {
 
 namespace {
@@ -66,6 +68,56 @@ LinearForm linear_form(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x
   // but 24 x 2048 -> 5120 6.6, 9.1; one row 2048 -> 5120 4.4, 6.8.
   const int64_t row_bytes = (w.in_features + 63) / 64 * 64 * (int64_t)dtype_size(x_dtype);
   return rows * 16 * row_bytes > 256 * 1024 ? LinearForm::kSplit : LinearForm::kOne;
+}
+
+int decode_groups(int64_t cgs) {
+  // One column group per block while that is no more than a block per CU (one row 8192 ->
+  // 4096 7.7 us, two groups 10.8); above, two, which share the rows (24 x 2048 -> 5120 6.6, one 8.9)
+  return cgs <= 256 ? 1 : 2;
+}
+
+// The tile by how many there are, against 256 CUs. Times in us of tiles of 32 x 64, 64 x 64,
+// 64 x 128, 128 x 128 and 256 x 256, for n tiles of 128 x 128 (m of 256 x 256):
+//   1024 -> 512, 1024 rows (n = 32)  bf16 x int8   6.2   7.4   9.9  13.8  28.4
+//   4096 -> 2048, 333 (48)           bf16 x int8  19.6  18.6  26.8  39.3  83.6
+//   2560 -> 6144, 200 / 512 (96, 192)       bf16  19.7 / 35.5, 16.4 / 26.6, 23.0 / 25.3, 27.5 / 28.0
+//   4096 -> 2048, 1500 (192)         bf16 x int8  46.6  34.5  37.2  39.9  84.3
+//   2048 -> 5120, 700 (240)          bf16 x int8  28.8  25.2  22.5  24.6  48.8
+//   4096 -> 9216, 333 / 512 (216, 288)      int8  32.7 / 42.6, 26.2 / 33.3, 22.0 / 29.3, 25.3 / 33.3
+//   2560 -> 6144, 1024 (384)                bf16  62.3  48.6  39.4  40.3  59.3
+//   2048 -> 5120, 1500 (480)                bf16  63.7  47.9  43.0  34.7  51.2
+//   2048 -> 5120, 2048 (640; m = 160) bf16 x int8 74.6  55.5  47.9  48.6  55.3
+//   2560 -> 6144, 2048 (768; m = 192)       bf16 119.7  93.6  74.2  70.1  64.2
+//   4096 -> 9216, 2048 (1152; m = 288)      int8 153.3 111.7  90.2  87.6  75.6 (quarters in the last round)
+// A tile is not much taller than the rows: 64 rows 2048 -> 151936 in tiles of 256 rows 152 us,
+// of 64 114; 300 x 4096 -> 9216 in tiles of 256 46.9, of 128 37.7; but 160 x 2048 -> 151936 166, 182.
+// With adapters, of which a low tile meets fewer, 32 x 64 up to 96 tiles of 128 x 128: 128 rows
+// of as many requests, 64 adapters of rank 64, 2048 -> 5120 37.0 in tiles of 64, 29.2 of 32.
+LinearTile linear_tile(int64_t tokens, int64_t cgs, bool converts, bool lora) {
+  const int64_t tm = (tokens + 255) / 256, tn = (cgs + 15) / 16;
+  const int64_t mid = ((tokens + 127) / 128) * ((cgs + 7) / 8);
+  if (tm * tn >= 176 && tm * 256 * 3 <= tokens * 5) return LinearTile::k256x256;
+  if (mid >= 400 && tokens > 64) return LinearTile::k128x128;
+  if (mid >= (converts ? 224 : 144) && tokens > 32) return LinearTile::k64x128;
+  if (mid > (lora ? 96 : 32) && tokens > 32) return LinearTile::k64x64;
+  return LinearTile::k32x64;
+}
+
+LinearRounds linear_rounds(int64_t tiles) {
+  // what is left after the whole rounds goes in quarters, unless those would take four rounds
+  const int64_t rest = tiles % 256;
+  if (tiles > 256 && rest <= 192) return {tiles - rest, tiles - rest + (4 * rest + 7) / 8 * 8};
+  const int64_t whole = (tiles + 7) / 8 * 8;
+  return {whole, whole};
+}
+
+LoraShrink lora_shrink(int64_t tokens, int64_t rank, int64_t adapters) {
+  // one block per CU: what the tiles leave of them goes to the groups, then to the adapters (up to
+  // two per CU was no faster for 128 rows and cost 4096 rows 2 us)
+  const int64_t tiles = (tokens + 15) / 16, groups = (rank + 15) / 16, room = std::max<int64_t>(256 / tiles, 1);
+  const int64_t ng = groups <= room ? 1 : (groups <= 2 ? 2 : 4);
+  const int64_t z = std::min((groups + ng - 1) / ng, room), y = std::min({room / z, (int64_t)16, adapters});
+  return {(int)ng, (unsigned)y, (unsigned)z};
 }
 
 LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora,
