@@ -265,6 +265,8 @@ def linear(
         if v.stride(1) != 1 or v.stride(0) < K:
             v = v.contiguous()
     stride = v.stride(0) if T > 1 else K
+    if stride > K and T * stride * v.element_size() >= 1 << 32:  # past the kernels' offsets
+        v, stride = v.contiguous(), K
     if (lora is None) != (batch is None):
         raise ValueError("lora and batch come together")
     ls = bs = None
