@@ -47,8 +47,17 @@ def _elsewhere(device: torch.device) -> bool:
     return device.index != torch._C._cuda_getDevice()
 
 
+def _require_buffer(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, device: torch.device) -> int:
+    """The address of a buffer that the kernels take for ``n`` elements."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < n:
+        what = f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} elements on {device} (got {what})")
+    return t.data_ptr()
+
+
 class _WithStruct:
-    """Keeps the C struct of a frozen dataclass after its first use; copies make their own."""
+    """Keeps the C struct of a frozen dataclass after its first use, which checks that the buffers
+    hold what the sizes say; copies make their own."""
 
     def __getstate__(self):
         state = dict(self.__dict__)
@@ -67,10 +76,16 @@ class PackedLinear(_WithStruct):
 
     @cached_property
     def struct(self) -> _lib.KmoeLinear:
-        code = _lib.DTYPE_I8 if self.values.dtype == torch.int8 else _lib.DTYPE_BF16
-        return _lib.KmoeLinear(
-            self.values.data_ptr(), self.scale.data_ptr(), code, self.in_features, self.out_features
-        )
+        dev, dtype = self.values.device, self.values.dtype
+        if dtype not in (torch.int8, torch.bfloat16):
+            raise ValueError(f"the packed values must be int8 or bfloat16 (got {dtype})")
+        code = _lib.DTYPE_I8 if dtype == torch.int8 else _lib.DTYPE_BF16
+        st = _lib.KmoeLinear(None, None, code, self.in_features, self.out_features)
+        nv, ns = ctypes.c_size_t(), ctypes.c_size_t()
+        _lib.check(_lib.lib().kmoe_linear_pack_bytes(st, ctypes.byref(nv), ctypes.byref(ns)))
+        st.values = _require_buffer(self.values, "values", dtype, nv.value // dtype.itemsize, dev)
+        st.scale = _require_buffer(self.scale, "scale", torch.float32, ns.value // 4, dev)
+        return st
 
     @property
     def nbytes(self) -> int:
@@ -117,10 +132,14 @@ class LoraAdapters(_WithStruct):
 
     @cached_property
     def struct(self) -> _lib.KmoeLora:
-        return _lib.KmoeLora(
-            self.a.data_ptr(), self.b.data_ptr(), self.factor.data_ptr(), self.num_adapters, self.rank,
-            self.in_features, self.out_features,
-        )  # fmt: skip
+        dev = self.a.device
+        st = _lib.KmoeLora(None, None, None, self.num_adapters, self.rank, self.in_features, self.out_features)
+        na, nb = ctypes.c_size_t(), ctypes.c_size_t()
+        _lib.check(_lib.lib().kmoe_lora_pack_bytes(st, ctypes.byref(na), ctypes.byref(nb)))
+        st.a = _require_buffer(self.a, "a", torch.bfloat16, na.value // 2, dev)
+        st.b = _require_buffer(self.b, "b", torch.bfloat16, nb.value // 2, dev)
+        st.factor = _require_buffer(self.factor, "factor", torch.float32, self.num_adapters, dev)
+        return st
 
     @staticmethod
     def empty(
@@ -195,7 +214,8 @@ class LoraBatch(_WithStruct):
 
     @cached_property
     def struct(self) -> _lib.KmoeLoraBatch:
-        p, n = self.buffer.data_ptr(), 4 * self.tokens
+        count = 3 * self.tokens + self.num_adapters + 1
+        p, n = _require_buffer(self.buffer, "buffer", torch.int32, count, self.buffer.device), 4 * self.tokens
         return _lib.KmoeLoraBatch(p, p + n, p + 2 * n, p + 3 * n, self.tokens, self.num_adapters)
 
 
