@@ -375,7 +375,8 @@ kmoe_status kmoe_linear_call_bytes(const kmoe_linear_weight* w, int64_t tokens, 
  * bf16(u) + bf16(u - bf16(u)) above. A row's bits depend on its own x and adapter and on T, not
  * on the other rows; a row whose x or u is not finite (u: in bf16) comes out not finite, as infinity or NaN.
  * workspace may be NULL where kmoe_linear_call_bytes gives 0; calls that may run at once need
- * one each. lora and batch are both NULL or both given. x spans less than 4 GiB. */
+ * one each. out and the workspace overlap neither each other nor x's rows. lora and batch are both
+ * NULL or both given. x spans less than 4 GiB. */
 kmoe_status kmoe_linear(const kmoe_linear_weight* w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
                         int64_t x_stride, const float* x_scale, const kmoe_lora* lora, const kmoe_lora_batch* batch,
                         void* out, void* workspace, size_t workspace_bytes, void* stream);

@@ -91,5 +91,8 @@ kmoe_status validate_linear(const kmoe_linear_weight* w, int64_t tokens, const v
                             int64_t x_stride, const float* x_scale, const kmoe_lora* lora,
                             const kmoe_lora_batch* batch, const void* out, const void* workspace,
                             size_t workspace_bytes, LinearSpace* space);
+// That out and the workspace overlap neither x's rows nor each other (tokens > 0, the call valid otherwise)
+kmoe_status validate_linear_apart(const kmoe_linear_weight& w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                                  int64_t x_stride, const void* out, const void* workspace, const LinearSpace& space);
 
 }  // namespace kmoe_host

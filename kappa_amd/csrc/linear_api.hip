@@ -68,6 +68,7 @@ kmoe_status kmoe_linear(const kmoe_linear_weight* w, int64_t tokens, const void*
                            &space));
   KMOE_TRY(kmoe_device_check());
   if (tokens == 0) return KMOE_OK;
+  KMOE_TRY(validate_linear_apart(*w, tokens, x, x_dtype, x_stride, out, workspace, space));
   return launched(launch_linear(*w, tokens, x, x_dtype, x_stride, x_scale, lora, batch, out, workspace, space,
                                 (hipStream_t)stream),
                   "linear kernels");

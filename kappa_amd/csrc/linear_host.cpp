@@ -315,4 +315,28 @@ kmoe_status validate_linear(const kmoe_linear_weight* w, int64_t tokens, const v
   return KMOE_OK;
 }
 
+namespace {
+
+// n bytes at p against `rows` stretches of `row` bytes, `pitch` >= row apart from x on
+bool meets(const void* p, size_t n, const void* x, size_t rows, size_t row, size_t pitch) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(x);
+  if (n == 0 || rows * row == 0 || a + n <= b) return false;
+  // the first row that ends behind p; it or none
+  const size_t first = a >= b + row ? (a - b - row) / pitch + 1 : 0;
+  return first < rows && b + first * pitch < a + n;
+}
+
+}  // namespace
+
+kmoe_status validate_linear_apart(const kmoe_linear_weight& w, int64_t tokens, const void* x, kmoe_dtype x_dtype,
+                                  int64_t x_stride, const void* out, const void* workspace, const LinearSpace& space) {
+  const size_t size = dtype_size(x_dtype), rows = (size_t)tokens, row = (size_t)w.in_features * size;
+  const size_t pitch = (size_t)x_stride * size, n = 2 * rows * (size_t)w.out_features;
+  if (meets(out, n, x, rows, row, pitch) || meets(out, n, workspace, 1, space.total, space.total))
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_linear: out must not overlap x or the workspace");
+  if (meets(workspace, space.total, x, rows, row, pitch))
+    return fail(KMOE_ERR_INVALID_ARG, "kmoe_linear: the workspace must not overlap x");
+  return KMOE_OK;
+}
+
 }  // namespace kmoe_host

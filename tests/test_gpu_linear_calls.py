@@ -3,6 +3,8 @@ rows far apart, buffers that do not fit, buffers that overlap."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -31,3 +33,35 @@ def test_rows_that_span_4_gib_or_more(dev, rows):
     far = torch.empty((T - 1) * stride + K, dtype=v.dtype, device=dev).as_strided((T, K), (stride, 1))
     far.copy_(v)
     assert torch.equal(linear(Q8Rows(far, x.scale) if rows == "q8" else far, p), linear(x, p))
+
+
+def test_buffers_that_overlap_are_refused(dev):
+    """C ABI: out on the rows, on the workspace, and the workspace on the rows; beside them, and
+    in the gap between two rows, is fine."""
+    from kappa_amd import _lib
+    from kappa_amd.qwen3 import linear, prepack_linear
+    from kappa_amd.qwen3.projection import _stream
+
+    T, K, N = 2, 250, 96  # rows that are copied into the workspace
+    x, w, _, _ = make(dev, T, K, N)
+    p = prepack_linear(w)
+    L, n = _lib.lib(), ctypes.c_size_t()
+    rows = torch.zeros(T, 2048, dtype=torch.bfloat16, device=dev)
+    rows[:, :K] = x
+    _lib.check(L.kmoe_linear_call_bytes(p.struct, T, rows.data_ptr(), _lib.DTYPE_BF16, 2048, None, ctypes.byref(n)))
+    assert 0 < n.value <= 2048
+    ws, out = torch.empty(n.value, dtype=torch.uint8, device=dev), torch.empty(T, N, dtype=torch.bfloat16, device=dev)
+
+    def call(o, s):
+        return L.kmoe_linear(p.struct, T, rows.data_ptr(), _lib.DTYPE_BF16, 2048, None, None, None, o, s, n.value, _stream(dev))
+
+    at, gap = rows.data_ptr(), rows.data_ptr() + 2 * 256
+    assert call(at, ws.data_ptr()) == _lib.ERR_INVALID_ARG
+    assert call(at + 4096 - 2, ws.data_ptr()) == _lib.ERR_INVALID_ARG
+    assert call(ws.data_ptr(), ws.data_ptr()) == _lib.ERR_INVALID_ARG
+    assert call(out.data_ptr(), at) == _lib.ERR_INVALID_ARG
+    want = linear(x, p)
+    _lib.check(call(out.data_ptr(), ws.data_ptr()))
+    assert torch.equal(out, want)
+    _lib.check(call(gap, gap + 1024))
+    assert torch.equal(rows[0, 256 : 256 + T * N].view(T, N), want) and torch.equal(rows[:, :K], x)

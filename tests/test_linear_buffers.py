@@ -1,13 +1,18 @@
 """Packed weights, adapters and batches whose fields do not belong together (made by hand or by
 dataclasses.replace) are refused before a kernel reads past a buffer (CPU: the check needs no
-device)."""
+device); and so are an output and a workspace that overlap the rows or each other."""
 
 from __future__ import annotations
 
 import dataclasses
+import os
+import shutil
 
 import pytest
 import torch
+
+from conftest import ROOT
+from test_host_sanitized import _build, _run
 
 from kappa_amd.qwen3 import LoraAdapters, LoraBatch, PackedLinear
 
@@ -64,3 +69,11 @@ def test_what_fits_is_taken(make):
 def test_what_does_not_fit_is_refused(make, over, match):
     with pytest.raises(ValueError, match=match):
         dataclasses.replace(make(), **over).struct
+
+
+@pytest.mark.skipif(shutil.which(os.environ.get("CXX", "g++")) is None, reason="no C++ compiler")
+def test_overlaps(tmp_path):
+    src = [os.path.join(ROOT, "kappa_amd", "csrc", f) for f in ("host.cpp", "linear_host.cpp")]
+    exe = _build(tmp_path, [*src, os.path.join(ROOT, "tests", "sanitize", "linear_apart.cpp")], "linear_apart")
+    r = _run(exe)
+    assert r.returncode == 0 and "linear apart: ok" in r.stdout, r.stdout + r.stderr
