@@ -11,6 +11,8 @@
 // h2 = round_act((f32(h) * r) * f32(scale)).
 #include <float.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "expert_dev.h"
 #include "launch.h"
@@ -303,20 +305,31 @@ using namespace kmoe;
 
 namespace {
 
+// Rows of one launch, `per` to a block: its threads are counted in 32 bits, and a launch of more
+// leaves the rows behind them out without an error.
+int64_t launch_rows(int per) { return (((int64_t)1 << 32) / (64 * kNormWaves) - 1) * per; }
+
 template <typename A, typename S, int W>
 void add_rms_norm_of(const kmoe_desc& d, const void* x, const void* res, const void* scale, float eps, void* hout,
                      void* out, int8_t* q, float* qscale, hipStream_t st) {
-  const int T = (int)d.tokens, D = (int)d.hidden, per = kNormWaves / W;
-  const dim3 grid((T + per - 1) / per), block(64 * kNormWaves);
+  const int D = (int)d.hidden, per = kNormWaves / W;
   const size_t lds = per * NormRow<A>::bytes(D);
-  if (q)
-    hipLaunchKernelGGL((k_add_rms_norm<A, S, true, W>), grid, block, lds, st, T, D, eps, reinterpret_cast<const A*>(x),
-                       reinterpret_cast<const A*>(res), reinterpret_cast<const S*>(scale), reinterpret_cast<A*>(hout),
-                       reinterpret_cast<A*>(out), q, qscale);
-  else
-    hipLaunchKernelGGL((k_add_rms_norm<A, S, false, W>), grid, block, lds, st, T, D, eps, reinterpret_cast<const A*>(x),
-                       reinterpret_cast<const A*>(res), reinterpret_cast<const S*>(scale), reinterpret_cast<A*>(hout),
-                       reinterpret_cast<A*>(out), q, qscale);
+  const int64_t most = launch_rows(per);
+  for (int64_t t = 0; t < d.tokens; t += most) {
+    const int T = (int)std::min(d.tokens - t, most);
+    const dim3 grid((T + per - 1) / per), block(64 * kNormWaves);
+    auto rows = [&](auto* p) { return p ? p + t * D : nullptr; };
+    const A* const xt = rows(reinterpret_cast<const A*>(x));
+    const A* const rt = rows(reinterpret_cast<const A*>(res));
+    A* const ht = rows(reinterpret_cast<A*>(hout));
+    A* const ot = rows(reinterpret_cast<A*>(out));
+    if (q)
+      hipLaunchKernelGGL((k_add_rms_norm<A, S, true, W>), grid, block, lds, st, T, D, eps, xt, rt,
+                         reinterpret_cast<const S*>(scale), ht, ot, rows(q), qscale + t);
+    else
+      hipLaunchKernelGGL((k_add_rms_norm<A, S, false, W>), grid, block, lds, st, T, D, eps, xt, rt,
+                         reinterpret_cast<const S*>(scale), ht, ot, q, qscale);
+  }
 }
 
 template <typename A, typename S>
@@ -350,29 +363,36 @@ hipError_t launch_add_rms_norm(const kmoe_desc& d, const void* x, const void* re
   return hipGetLastError();
 }
 
+namespace {
+
+template <typename A, typename S>
+void rms_norm_of(const kmoe_desc& d, const void* h, const void* scale, float eps, void* out, hipStream_t st) {
+  const int D = (int)d.hidden;
+  const int64_t most = launch_rows(kNormWaves);
+  for (int64_t t = 0; t < d.tokens; t += most) {
+    const int T = (int)std::min(d.tokens - t, most);
+    hipLaunchKernelGGL((k_rms_norm<A, S>), dim3((T + kNormWaves - 1) / kNormWaves), dim3(64 * kNormWaves),
+                       kNormWaves * NormRow<A>::bytes(D), st, T, D, eps, reinterpret_cast<const A*>(h) + t * D,
+                       reinterpret_cast<const S*>(scale), reinterpret_cast<A*>(out) + t * D);
+  }
+}
+
+}  // namespace
+
 hipError_t launch_rms_norm(const kmoe_desc& d, const void* h, const void* scale, kmoe_dtype scale_dtype, float eps,
                            void* out, hipStream_t st) {
-  const int T = (int)d.tokens, D = (int)d.hidden;
-  if (T == 0) return hipSuccess;
-  const dim3 grid((T + kNormWaves - 1) / kNormWaves);
-  const bool act_bf16 = d.act_dtype == KMOE_DTYPE_BF16, s_bf16 = scale_dtype == KMOE_DTYPE_BF16;
-  const size_t lds = kNormWaves * (act_bf16 ? NormRow<uint16_t>::bytes(D) : NormRow<float>::bytes(D));
-  if (act_bf16 && s_bf16)
-    hipLaunchKernelGGL((k_rms_norm<uint16_t, uint16_t>), grid, dim3(64 * kNormWaves), lds, st, T, D, eps,
-                       reinterpret_cast<const uint16_t*>(h), reinterpret_cast<const uint16_t*>(scale),
-                       reinterpret_cast<uint16_t*>(out));
-  else if (act_bf16)
-    hipLaunchKernelGGL((k_rms_norm<uint16_t, float>), grid, dim3(64 * kNormWaves), lds, st, T, D, eps,
-                       reinterpret_cast<const uint16_t*>(h), reinterpret_cast<const float*>(scale),
-                       reinterpret_cast<uint16_t*>(out));
-  else if (s_bf16)
-    hipLaunchKernelGGL((k_rms_norm<float, uint16_t>), grid, dim3(64 * kNormWaves), lds, st, T, D, eps,
-                       reinterpret_cast<const float*>(h), reinterpret_cast<const uint16_t*>(scale),
-                       reinterpret_cast<float*>(out));
-  else
-    hipLaunchKernelGGL((k_rms_norm<float, float>), grid, dim3(64 * kNormWaves), lds, st, T, D, eps,
-                       reinterpret_cast<const float*>(h), reinterpret_cast<const float*>(scale),
-                       reinterpret_cast<float*>(out));
+  const bool s_bf16 = scale_dtype == KMOE_DTYPE_BF16;
+  if (d.act_dtype == KMOE_DTYPE_BF16) {
+    if (s_bf16)
+      rms_norm_of<uint16_t, uint16_t>(d, h, scale, eps, out, st);
+    else
+      rms_norm_of<uint16_t, float>(d, h, scale, eps, out, st);
+  } else {
+    if (s_bf16)
+      rms_norm_of<float, uint16_t>(d, h, scale, eps, out, st);
+    else
+      rms_norm_of<float, float>(d, h, scale, eps, out, st);
+  }
   return hipGetLastError();
 }
 

@@ -174,6 +174,30 @@ def test_in_place(dev):
             assert torch.equal(at, h) and torch.equal(qv, q.values) and torch.equal(qs, q.scale)
 
 
+@pytest.mark.parametrize("T,D", [((1 << 24) + 5, 1032), ((1 << 26) + 5, 8)])
+def test_more_rows_than_one_launch_takes(dev, T, D):
+    """A launch holds less than 2^32 threads: 2^24 rows of 256, 2^26 of 64. Rows repeat after 1009."""
+    from kappa_amd.qwen3 import add_rms_norm, add_rms_norm_q8, rms_norm
+
+    x, res, scale = _case(dev, 1009, D, "bf16", "bf16", 9)
+    many = x.repeat(-(-T // 1009), 1)[:T]
+    q, s = add_rms_norm_q8(many, None, scale)[0]
+    want = add_rms_norm_q8(x, None, scale)[0]
+    for t in (0, 12345, T - 2018 - T % 1009, T - 1009 - T % 1009):
+        a = -t % 1009 + t  # where the pattern starts
+        n = min(1009, T - a)
+        assert torch.equal(q[a : a + n], want.values[:n]) and torch.equal(s[a : a + n], want.scale[:n])
+    n = T % 1009
+    assert torch.equal(q[T - n :], want.values[:n]) and torch.equal(s[T - n :], want.scale[:n])
+    if D == 8:
+        normed, h = add_rms_norm(many, res.repeat(-(-T // 1009), 1)[:T], scale)
+        want, hw = add_rms_norm(x, res, scale)
+        assert torch.equal(normed[T - n :], want[:n]) and torch.equal(h[T - n :], hw[:n])
+        assert torch.equal(normed[:1009], want) and torch.equal(h[:1009], hw)
+        normed, want = rms_norm(many, scale), rms_norm(x, scale)
+        assert torch.equal(normed[T - n :], want[:n]) and torch.equal(normed[:1009], want)
+
+
 def test_no_rows(dev):
     from kappa_amd.qwen3 import add_rms_norm, add_rms_norm_q8
 
