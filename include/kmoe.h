@@ -372,8 +372,10 @@ kmoe_status kmoe_linear_call_bytes(const kmoe_linear_weight* w, int64_t tokens, 
  *           x_scale [T] f32 (kmoe_add_rms_norm_q8's outputs), which takes I8 weights
  *   out     [T, out] BF16
  * Sums in f32 (int8 rows: exact in i32 first); u stays f32 up to 64 tokens and is carried as
- * bf16(u) + bf16(u - bf16(u)) above. A row's bits depend on its own x and adapter and on T, not
- * on the other rows; a row whose x or u is not finite (u: in bf16) comes out not finite, as infinity or NaN.
+ * bf16(u) + bf16(u - bf16(u)) above. A row's bits depend on its own x and adapter, on T and, up to
+ * 64 tokens, on whether lora is given (the sums then run in another order, those of rows without an
+ * adapter too), not on the other rows: given in every call, it keeps a request's bits whatever the
+ * others use. A row whose x or u is not finite (u: in bf16) comes out not finite, as infinity or NaN.
  * workspace may be NULL where kmoe_linear_call_bytes gives 0; calls that may run at once need
  * one each. out and the workspace overlap neither each other nor x's rows. lora and batch are both
  * NULL or both given. x spans less than 4 GiB. */

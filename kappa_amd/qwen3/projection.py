@@ -251,7 +251,9 @@ def linear(
     """``x @ w`` with the adapters of each token's request: ``[..., in]`` -> bf16 ``[..., out]``.
 
     ``x`` is bf16, or 8-bit rows (which need int8 weights). Sums are f32 (8-bit rows: exact),
-    rounded once at the end. A row's bits do not depend on the other rows' adapters."""
+    rounded once at the end. A row's bits do not depend on the other rows' adapters; up to 64
+    tokens they do depend on whether ``lora`` is given at all, so a server whose requests may use
+    adapters passes it on every step, also where all tokens have -1."""
     if not isinstance(w, PackedLinear):
         raise ValueError(f"w must be a PackedLinear from prepack_linear (got {type(w).__name__})")
     K = w.in_features
