@@ -45,9 +45,28 @@ bool linear_rows_fit(const kmoe_linear_weight& w, const void* x, kmoe_dtype x_dt
          x_stride * (int64_t)dtype_size(x_dtype) % 16 == 0;
 }
 
+// Blocks that share the reduction of a row in the two-launch form: each leaves its partial sums
+static int64_t split_parts(const kmoe_linear_weight& w, kmoe_dtype x_dtype) {
+  return (padded_in(w.in_features) / step_of(x_dtype) + kmoe::kSplitSteps - 1) / kmoe::kSplitSteps;
+}
+
 LinearForm linear_form(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, bool lora) {
   if (tokens > kmoe::kLinearDecodeTokens) return LinearForm::kTiles;
-  if (lora) return LinearForm::kSplit;
+  // The partial sums of two launches stay below 64 MB: where they are more, tiles are as fast or
+  // faster for the most part, and the workspace would grow with in x out (34 GB at the limits).
+  // us (two launches, tiles), bf16 / bf16 x int8 / int8, 16 adapters of rank 16:
+  //   64 x 2048 -> 151936 (156, 156, 78 MB)   215, 149 / 180, 103 / 132, 103
+  //   64 x 4096 -> 65536  (134, 134, 67 MB)   163, 125 / 133,  77 /  89,  72
+  //   64 x 4096 -> 32768   (67,  67, 34 MB)    87,  85 /  73,  52 /  52,  52
+  //   64 x 8192 -> 28672  (117, 117, 59 MB)   138, 146 / 116,  83 /  76,  80
+  //   64 x 4096 -> 9216    (19,  19,  9 MB)    32,  40 /  28,  30 /  22,  23
+  //   24 x 2048 -> 16384  (6.3, 6.3, 3 MB)     23,  22 /  18,  20 /  15,  18
+  //    8 x 2048 -> 5120                      10.6, 14.8 / 8.9, 15.9 / 9.1, 12.5
+  // without adapters, 16 x 16384 -> 32768 (67, 67, 34 MB) 221, 184 / 112, 96 / 102, 96; 16 x 32768 ->
+  // 16384 (the same) 187, 179 / 109, 122 / 97, 93; one row of it 164, 179 / 91, 121 / 85, 92.
+  const int64_t sums = split_parts(w, x_dtype) * tokens * padded_out(w.out_features) * 4;
+  const LinearForm two = sums < ((int64_t)64 << 20) ? LinearForm::kSplit : LinearForm::kTiles;
+  if (lora) return two;
   // Above 16 rows the one launch grows with the 16-row groups times the column groups, the tiles
   // do not. us (one or two launches, tiles), bf16 / bf16 x int8 / int8:
   //   17 x 4096 -> 9216   (1152)   23.7, 14.0 /  18.0, 15.2 /  12.7, 9.2
@@ -56,9 +75,12 @@ LinearForm linear_form(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x
   //   64 x 2048 -> 5120   (1280)   12.8,  9.8 /  11.5, 10.6 /   8.3, 7.2
   //   64 x 4096 -> 2048    (512)   12.3, 14.0 /  10.8, 15.2 /  12.0, 8.6
   //   64 x 2048 -> 151936 (37984)  210,   114 /   188, 68   /   134, 65
-  // Up to 16 rows: 16 x 2048 -> 16384 13.5, 12.3 / 9.7, 9.6 / 8.7, 8.1; one row -> 151936 93,
-  // 102 / 51, 55 / 49, 53; but where the one launch's blocks (of two column groups) make a
-  // full round of 256 CUs and a small one, 4096 -> 9216, one row 18.6, 13.5 / 10.3, 14.6 / 9.2, 8.7.
+  // Up to 16 rows the one launch (one row -> 151936 93, 102 / 51, 55 / 49, 53), but where its blocks
+  // (of two column groups) make a full round of 256 CUs and a small one: 4096 -> 9216, one row
+  // 18.6, 13.5 / 10.3, 14.6 / 9.2, 8.7. Wider ones stay with it for one row's sake, though 16 rows
+  // are faster in tiles up to about 1300 groups: 2048 -> 12288 (768), one row 10.8, 10.0 / 7.3, 9.4 /
+  // 6.7, 7.0, 16 rows 13.0, 10.8 / 9.1, 9.7 / 8.0, 7.6; 2048 -> 24576 (1536) 17.5, 19.4 / 11.5, 11.5 /
+  // 10.1, 10.9 and 19.0, 20.3 / 15.1, 11.8 / 11.9, 11.0.
   const bool converts = enum_value(x_dtype) == KMOE_DTYPE_BF16 && enum_value(w.dtype) == KMOE_DTYPE_I8;
   const int64_t rows = (tokens + 15) / 16, columns = padded_out(w.out_features) / 16;
   if (rows > 1 ? rows * columns > (converts ? 1024 : 896) : !converts && columns > 512 && columns < 768)
@@ -67,7 +89,7 @@ LinearForm linear_form(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x
   // two), bf16 rows and int8 weights: 64 x 4096 -> 2048 18.4, 10.9; 64 x 8192 -> 4096 33.8, 23.6;
   // but 24 x 2048 -> 5120 6.6, 9.1; one row 2048 -> 5120 4.4, 6.8.
   const int64_t row_bytes = (w.in_features + 63) / 64 * 64 * (int64_t)dtype_size(x_dtype);
-  return rows * 16 * row_bytes > 256 * 1024 ? LinearForm::kSplit : LinearForm::kOne;
+  return rows * 16 * row_bytes > 256 * 1024 ? two : LinearForm::kOne;
 }
 
 int decode_groups(int64_t cgs) {
@@ -124,7 +146,7 @@ LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype
                          bool copied) {
   const size_t T = (size_t)tokens, in = (size_t)padded_in(w.in_features);
   const bool splits = linear_form(w, tokens, x_dtype, lora) == LinearForm::kSplit;
-  const size_t parts = (in / (size_t)step_of(x_dtype) + kmoe::kSplitSteps - 1) / kmoe::kSplitSteps;
+  const size_t parts = (size_t)split_parts(w, x_dtype);
   LinearSpace s;
   s.part = copied ? align256(T * in * dtype_size(x_dtype)) : 0;
   s.u = s.part + (splits ? align256(parts * T * (size_t)padded_out(w.out_features) * 4) : 0);
@@ -135,8 +157,8 @@ LinearSpace linear_space(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype
 
 size_t linear_most_bytes(const kmoe_linear_weight& w, int64_t tokens, kmoe_dtype x_dtype, const kmoe_lora* lora) {
   size_t most = linear_space(w, tokens, x_dtype, lora, true).total;
-  // fewer tokens may hold partial sums where these do not; the form changes with the 16-row groups
-  for (int64_t t = 16; t <= kmoe::kLinearDecodeTokens && t < tokens; t += 16) {
+  // fewer tokens may hold partial sums where these do not
+  for (int64_t t = 1; t <= kmoe::kLinearDecodeTokens && t < tokens; ++t) {
     const size_t s = linear_space(w, t, x_dtype, lora, true).total;
     if (s > most) most = s;
   }

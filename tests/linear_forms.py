@@ -31,6 +31,8 @@ SIZES = {
     (24, 4096, 257, 5, 40): "split 2 lora deep",
     (40, 2600, 130, 40, 8): "split 3 lora deep",
     (64, 4096, 2048, 16, 64): "split 4 lora deep",
+    # too many partial sums for two launches
+    (64, 1088, 140000, 3, 8): "64x128 lora deep, shrink 1",
     # tiles, their rings turning
     (129, 1216, 257, 0, 0): "32x64 deep",
     (80, 4200, 130, 3, 16): "32x64 lora deep, shrink 1 again",

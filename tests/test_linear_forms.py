@@ -4,6 +4,7 @@ change of a threshold cannot leave one without a test on the GPU."""
 
 from __future__ import annotations
 
+import ctypes
 import os
 import shutil
 import subprocess
@@ -11,6 +12,7 @@ import subprocess
 import pytest
 
 from conftest import ROOT
+from kappa_amd import _lib
 from linear_forms import KINDS, SIZES, names
 from test_host_sanitized import _build
 
@@ -57,3 +59,21 @@ def test_the_sizes_take_every_kernel(choose, k, kind):
     assert len({r.replace(" deep", "") for r in reached}) == KERNELS
     missing = {r for r in reached if r not in have and r + " deep" not in have}
     assert not missing, sorted(missing)
+
+
+def test_partial_sums_stay_bounded():
+    """The workspace of up to 64 tokens: the rows' copy, the adapters' inner values and less than
+    64 MB of partial sums, up to the largest weights."""
+    L = _lib.lib()
+    most, call = ctypes.c_size_t(), ctypes.c_size_t()
+    for K, N in ((2048, 151936), (4096, 65536), (65536, 1 << 20), (65536, 64), (16384, 32768)):
+        for R in (0, 16):
+            lora = _lib.KmoeLora(None, None, None, 4, R, K, N) if R else None
+            for dtype, x_dtype in ((_lib.DTYPE_BF16, _lib.DTYPE_BF16), (_lib.DTYPE_I8, _lib.DTYPE_BF16), (_lib.DTYPE_I8, _lib.DTYPE_I8)):
+                w = _lib.KmoeLinear(None, None, dtype, K, N)
+                need = 0
+                for T in range(1, 70):
+                    assert L.kmoe_linear_call_bytes(w, T, 0x1002, x_dtype, K, lora, call) == _lib.OK
+                    need = max(need, call.value)
+                    assert L.kmoe_linear_workspace_bytes(w, T, x_dtype, lora, most) == _lib.OK
+                    assert need <= most.value <= (64 << 20) + T * (2 * K + 4 * 32) + 1024
