@@ -509,14 +509,14 @@ __global__ __launch_bounds__(512) void k_linear_decode(LinearArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens in two launches (LinearForm::kSplit). The first: blocks of 128 columns and eight steps (128 bytes of
-// each row), every load of a block in flight at once - the rows through LDS, shared by NW
-// waves of 16 CG columns, the weights in registers - whose partial sums go to the workspace;
+// Few tokens in two launches (LinearForm::kSplit). The first: blocks of 128 columns, above 32 rows 64,
+// and eight steps (128 bytes of each row), every load of a block in flight at once - the rows through
+// LDS, shared by NW waves of 16 CG columns, the weights in registers - whose partial sums go to the workspace;
 // and beside them the blocks of the adapters' u, which thus costs no launch of its own. The
 // second adds the partial sums in order and the adapters' part, and rounds.
-// 64 rows with 32 adapters of rank 16, 2048 -> 5120: 14.2 us, of which the second 4; the
-// weights, adapters and rows alone would take 4 us of HBM. With u in a launch of its own and the
-// adapters' part in the single launch above it took 19.7.
+// 64 rows with 32 adapters of rank 16, 2048 -> 5120, int8 weights: 14.0 us, the first kernel 10.0 and
+// the second 4.7; the weights, adapters and rows alone would take 3.5 us of HBM. With u in a launch of
+// its own and the adapters' part in the single launch above it took 19.7.
 // ---------------------------------------------------------------------------
 template <int KIND, int RB, int NW, int CG>
 __global__ __launch_bounds__(64 * NW) void k_linear_split(LinearArgs p, int splits, int shrink_blocks) {
@@ -1033,9 +1033,9 @@ dim3 grid_for(int64_t items) {
 template <int KIND, int RB>
 void decode_of(const LinearArgs& p, bool split, hipStream_t st) {
   if (split) {
-    // Up to 32 rows bf16 rows take eight waves of 16 columns, int8 rows, which take half the LDS
-    // and no conversion, four of 32; above, where a block's rows fill more of the LDS, both
-    // take four of 16, so that more blocks run. us, 24 rows of rank 64, 4096 -> 9216: int8
+    // Up to 32 rows bf16 rows take eight waves of 16 columns, int8 rows, whose blocks cover twice the
+    // inputs in the same LDS and convert nothing, four of 32; above, where a block's rows fill more of
+    // the LDS, both take four of 16, so that more blocks run. us, 24 rows of rank 64, 4096 -> 9216: int8
     // weights 23.1 (four of 16 28.9), int8 rows 19.6 (28.2); 64 rows of rank 16, 4096 -> 2048, bf16
     // weights 16.3 with eight, 13.9 with four of 16, int8 rows 12.5 with four of 32, 11.0; 48 rows
     // 15.3, 13.1 and 11.5, 10.3.
