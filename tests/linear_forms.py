@@ -33,6 +33,9 @@ SIZES = {
     (64, 4096, 2048, 16, 64): "split 4 lora deep",
     # too many partial sums for two launches
     (64, 1088, 140000, 3, 8): "64x128 lora deep, shrink 1",
+    (32, 4600, 60000, 3, 8): (
+        "32x64 lora deep, shrink 1 again", "32x64 lora deep, shrink 1 again", "split 2 lora deep",
+    ),
     # tiles, their rings turning
     (129, 1216, 257, 0, 0): "32x64 deep",
     (80, 4200, 130, 3, 16): "32x64 lora deep, shrink 1 again",

@@ -1,5 +1,5 @@
 """Calls of ``linear`` that its documentation allows and whose form is out of the ordinary (GPU):
-rows far apart, buffers that do not fit, buffers that overlap."""
+rows far apart, buffers that overlap, the largest sizes."""
 
 from __future__ import annotations
 
@@ -8,7 +8,8 @@ import ctypes
 import pytest
 import torch
 
-from test_gpu_linear import make
+from linear_forms import KINDS
+from test_gpu_linear import check, make, make_adapters
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +66,38 @@ def test_buffers_that_overlap_are_refused(dev):
     assert torch.equal(out, want)
     _lib.check(call(gap, gap + 1024))
     assert torch.equal(rows[0, 256 : 256 + T * N].view(T, N), want) and torch.equal(rows[:, :K], x)
+
+
+LIMITS = [(1 << 20, 64, 40, 5, 8), (3, 64, 1 << 20, 2, 8), (70, 64, 1 << 20, 0, 0), (1, 65536, 32, 3, 16), (70, 65536, 32, 3, 16),
+          (40, 128, 32, 1024, 256), (1100, 128, 32, 1024, 256)]  # fmt: skip
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,K,N,L,R", LIMITS)
+def test_the_largest_sizes(dev, T, K, N, L, R, kind):
+    """The limits of tokens, inputs, outputs, adapters and rank, one or two at a time."""
+    from kappa_amd.qwen3 import linear, lora_batch, prepack_linear, prepack_lora
+
+    x, w, xd, wd = make(dev, T, K, N, *KINDS[kind])
+    lora, kw = None, {}
+    if L:
+        lora = make_adapters(dev, T, K, N, L, R)
+        kw = dict(lora=prepack_lora(*lora[:3]), batch=lora_batch(lora[3], L))
+    check(linear(x, prepack_linear(w), **kw), xd, wd, K, lora, R)
+
+
+def test_one_more_than_the_largest_is_refused(dev):
+    from kappa_amd.qwen3 import LoraAdapters, linear, lora_batch, prepack_linear
+
+    def zeros(*shape, dtype=torch.bfloat16):
+        return torch.zeros(*shape, dtype=dtype, device=dev)
+
+    p = prepack_linear(zeros(8, 8))
+    for call in (
+        lambda: linear(zeros((1 << 20) + 1, 8), p), lambda: prepack_linear(zeros(65537, 1)),
+        lambda: prepack_linear(zeros(1, (1 << 20) + 1)), lambda: lora_batch(zeros((1 << 20) + 1, dtype=torch.int32), 1),
+        lambda: lora_batch(zeros(1, dtype=torch.int32), 1025), lambda: LoraAdapters.empty(1025, 1, 8, 8),
+        lambda: LoraAdapters.empty(1, 257, 8, 8), lambda: linear(zeros(1 << 20, 2048), prepack_linear(zeros(2048, 8))),
+    ):  # fmt: skip
+        with pytest.raises(ValueError):
+            call()
